@@ -57,6 +57,12 @@ extern "C" {
 #define NVMAI_ROUTER_AFFINE4 4u    /* affine codes + 16-bit scale/bias per 64 (moe.metal:157-214) */
 #define NVMAI_ROUTER_AFFINE8 8u
 #define NVMAI_GATE_NONE 0xFFFFFFFFu /* shared expert without a sigmoid gate */
+#define NVMAI_ACT_NONE 2u        /* int8_matmul only: no activation, no gate rows */
+/* element types of the row operators (sort_rows .. int8_matmul) */
+#define NVMAI_ELEM_F16 0u
+#define NVMAI_ELEM_F32 1u
+#define NVMAI_ELEM_BF16 2u
+#define NVMAI_ELEM_I8 3u         /* 8-bit codes with a scale per row */
 
 typedef struct nvmai_cuda_moe nvmai_cuda_moe;
 
@@ -441,6 +447,83 @@ NVMAI_API int nvmai_cuda_moe_affine_gemv(uint32_t bits, uint32_t meta_dtype, con
 NVMAI_API int nvmai_cuda_moe_silu_mul_f16(const void *gate, const void *up, void *out, uint32_t count, void *stream);
 NVMAI_API int nvmai_cuda_moe_sigmoid_scalar_mul_f16(void *y, const void *gate, uint32_t count, void *stream);
 NVMAI_API int nvmai_cuda_moe_residual_add_f16(void *hidden, const void *delta, uint32_t count, void *stream);
+
+/* ---- row operators: rows sorted by expert and back, products in 8-bit integers --------------
+ * For hosts that run experts of their own between router and sum (other weights, adapters,
+ * training of router and inputs), or experts stored as symmetric 8-bit integers.  No counterpart
+ * in the reference.  No handle: every buffer is the caller's, nothing is allocated, no state is
+ * kept between calls, and calls on different streams are independent as long as their buffers
+ * (workspaces included) are.  Calls can be captured.  Strides count elements (codes: bytes) from
+ * one row to the next and are at least the row's length.  All pointers belong to the current
+ * device (NVMAI_CUDA_EINVAL otherwise); indexes and positions are checked on the device, an
+ * entry out of range counts as not held, never as an address. */
+
+/* Sorts the tokens * top_k pairs (token t, slot k), pair = t * top_k + k, by expert: pairs with
+ * idx[pair] < num_experts are kept, ordered by (expert, pair); the others (a padded row's, another
+ * rank's experts) are not.
+ *   position[pair]  its row in that order, or 0xFFFFFFFF
+ *   source[row]     the pair of a row; 0xFFFFFFFF from row expert_begin[num_experts] on
+ *   expert_begin[e] first row of expert e; [num_experts] = number of kept pairs
+ * With x (tokens rows of d elements) and rows it also brings each kept pair's token row to its place;
+ * rows behind the last kept one are left as they were.  rows_elem is x_elem (a copy of the bits),
+ * or NVMAI_ELEM_I8: codes and row_scales as nvmai_cuda_moe_quantize_rows makes them.  x = rows =
+ * NULL: the order alone.  top_k <= 64, num_experts <= 1024, tokens * top_k < 2^31; tokens = 0 is
+ * valid.  The gradient of x is nvmai_cuda_moe_merge_rows of the rows' gradient, without weights.
+ * workspace: device memory, as many bytes as _sort_rows_workspace says (0 for small calls). */
+NVMAI_API uint64_t nvmai_cuda_moe_sort_rows_workspace(uint32_t tokens, uint32_t top_k, uint32_t num_experts);
+NVMAI_API int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_k, uint32_t num_experts,
+                                       uint32_t *position, uint32_t *source, uint32_t *expert_begin, const void *x,
+                                       uint32_t x_elem, uint32_t x_stride, uint32_t d, void *rows, uint32_t rows_elem,
+                                       uint32_t rows_stride, float *row_scales, void *workspace,
+                                       uint64_t workspace_bytes, void *stream);
+
+/* y[t] = base[t] + sum over k of w[t][k] * rows[position[t][k]]: expert rows back to their tokens,
+ * in fp32 with k ascending, rounded once.  Positions >= n_rows add nothing, whatever their weight
+ * is; w = NULL: weights of 1 (the gradient of sort_rows); base = NULL: 0.  rows, base and y have the type
+ * `elem` (F16, F32, BF16), w has w_elem.  y may be base itself (the same rows in place). */
+NVMAI_API int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_t rows_stride, uint32_t n_rows,
+                                        const uint32_t *position, const void *w, uint32_t w_elem, uint32_t tokens,
+                                        uint32_t top_k, uint32_t d, const void *base, uint32_t base_stride, void *y,
+                                        uint32_t y_stride, void *stream);
+
+/* Gradients of merge_rows: drows[position[t][k]] = w[t][k] * dy[t] (rounded to `elem`; rows that no
+ * position names are left as they were) and dw[t][k] = sum over i of dy[t][i] * rows[position[t][k]][i]
+ * (fp32; 0 where the position is not held).  w = NULL: weights of 1.  Either of drows and dw may be NULL;
+ * rows may be NULL without dw; drows may be rows itself.  The gradient of base is dy. */
+NVMAI_API int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_stride, const void *rows,
+                                             uint32_t rows_stride, uint32_t n_rows, const uint32_t *position,
+                                             const void *w, uint32_t w_elem, uint32_t tokens, uint32_t top_k, uint32_t d,
+                                             void *drows, uint32_t drows_stride, float *dw, void *stream);
+
+/* Symmetric 8-bit codes of rows (activations by token, a matrix's rows by output channel):
+ *   m = max |x|, scales = m / 127, q = rint(x * (127 / m)), each step rounded to fp32, ties to even.
+ * A row whose m is below 2^-120 gets codes and a scale of 0; one that holds an infinity or a NaN gets codes of
+ * 0 and a scale of NaN, which makes every product with it NaN.  elem F16, F32 or BF16. */
+NVMAI_API int nvmai_cuda_moe_quantize_rows(const void *x, uint32_t elem, uint32_t x_stride, uint32_t rows, uint32_t n,
+                                           void *q, uint32_t q_stride, float *scales, void *stream);
+
+/* Products of rows with matrices of 8-bit codes [num_experts][channels][k] (rows b_stride bytes apart)
+ * that have a scale per channel, fp32 [num_experts][channels]:
+ *   v[r][j] = (a_scales[r] * b_scales[e][j]) * sum over i of a[r][i] * b[e][j][i]      (the sum exact, in 32-bit integers)
+ * activation NVMAI_ACT_NONE: channels = n, out[r][j] = v[r][j]; NVMAI_ACT_SILU / _GELU_TANH:
+ * channels = 2 n, gate rows before up rows, out[r][j] = act(v[r][j]) * v[r][n + j].  Rounded once to out_elem.
+ * expert_begin (u32 [num_experts + 1], ascending, as sort_rows writes it): rows begin[e] .. begin[e + 1] - 1
+ * are expert e's, rows of none are left as they were; NULL with num_experts = 1: all rows.
+ * a: codes with a_scales (NVMAI_ELEM_I8), or F16 / F32 / BF16 rows with a_scales = NULL, which the call
+ * quantises as quantize_rows does; these need a workspace of _int8_matmul_workspace bytes.
+ * Codes start on 16-byte boundaries and their strides are multiples of 16.  k < 131072 (the sum fits 32 bits);
+ * rows = 0 is valid.  Without an explicit wait of its own the call cannot report a device-side wait that gave up:
+ * nvmai_cuda_moe_int8_matmul_status does. */
+NVMAI_API uint64_t nvmai_cuda_moe_int8_matmul_workspace(uint32_t rows, uint32_t k, uint32_t a_elem);
+NVMAI_API int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride, const float *a_scales,
+                                         uint32_t rows, uint32_t k, const void *b, uint32_t b_stride,
+                                         const float *b_scales, uint32_t n, uint32_t num_experts,
+                                         const uint32_t *expert_begin, uint32_t activation, void *out, uint32_t out_elem,
+                                         uint32_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Waits for `stream`, then returns NVMAI_CUDA_ETIMEOUT if a bounded device-side wait of an int8_matmul call on the
+ * current device gave up since the last call of this function (the outputs of that product are undefined), else 0. */
+NVMAI_API int nvmai_cuda_moe_int8_matmul_status(void *stream);
 
 /* Optional per-kernel timeline of the single-token decode stages, the counterpart
  * of the reference's NVMAI_KERNEL_STATS command-buffer times

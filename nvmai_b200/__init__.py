@@ -9,3 +9,5 @@ loudly when the library is absent.
 from . import format, synthetic  # noqa: F401
 from .moe import (Elementwise, MoE, MoEConfig, NvmaiError, affine_gemv, dequant, launch_count,  # noqa: F401
                   router_noalloc)
+from .row_ops import (int8_matmul, int8_matmul_status, int8_matmul_workspace, merge_rows, merge_rows_grad,  # noqa: F401
+                      quantize_rows, sort_rows, sort_rows_workspace)

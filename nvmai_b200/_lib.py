@@ -84,6 +84,14 @@ PROTOTYPES = {
     "nvmai_cuda_moe_silu_mul_f16": (C.c_int, [vp, vp, vp, u32, vp]),
     "nvmai_cuda_moe_sigmoid_scalar_mul_f16": (C.c_int, [vp, vp, u32, vp]),
     "nvmai_cuda_moe_residual_add_f16": (C.c_int, [vp, vp, u32, vp]),
+    "nvmai_cuda_moe_sort_rows_workspace": (u64, [u32, u32, u32]),
+    "nvmai_cuda_moe_sort_rows": (C.c_int, [vp, u32, u32, u32, vp, vp, vp, vp, u32, u32, u32, vp, u32, u32, vp, vp, u64, vp]),
+    "nvmai_cuda_moe_merge_rows": (C.c_int, [vp, u32, u32, u32, vp, vp, u32, u32, u32, u32, vp, u32, vp, u32, vp]),
+    "nvmai_cuda_moe_merge_rows_grad": (C.c_int, [vp, u32, u32, vp, u32, u32, vp, vp, u32, u32, u32, u32, vp, u32, vp, vp]),
+    "nvmai_cuda_moe_quantize_rows": (C.c_int, [vp, u32, u32, u32, u32, vp, u32, vp, vp]),
+    "nvmai_cuda_moe_int8_matmul_workspace": (u64, [u32, u32, u32]),
+    "nvmai_cuda_moe_int8_matmul": (C.c_int, [vp, u32, u32, vp, u32, u32, vp, u32, vp, u32, u32, vp, u32, vp, u32, u32, vp, u64, vp]),
+    "nvmai_cuda_moe_int8_matmul_status": (C.c_int, [vp]),
     "nvmai_cuda_moe_set_trace": (C.c_int, [vp, C.c_int]),
     "nvmai_cuda_moe_read_trace": (C.c_int, [vp, vp, u32]),
     "nvmai_cuda_moe_read_block_trace": (C.c_int, [vp, vp, u32, C.POINTER(u32)]),

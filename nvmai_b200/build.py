@@ -14,7 +14,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libnvmai_cuda_moe.so"
-SOURCES = ["moe_api.cu", "batch_path.cu", "router_noalloc.cu"]
+SOURCES = ["moe_api.cu", "batch_path.cu", "router_noalloc.cu", "row_ops.cu", "int8_matmul.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--threads", "0", "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -1,11 +1,15 @@
 // Kernel launches of the library's translation units.
 #pragma once
 #include <cuda_runtime.h>
+#include <stdint.h>
 #include <map>
 #include <mutex>
 #include <utility>
 
 namespace nvmai {
+
+// Adds to nvmai_cuda_moe_launch_count (moe_api.cu).
+void count_launches(uint64_t launches);
 
 // Kernels here use more than the default 48 KB of dynamic shared memory; the
 // opt-in is per function and sticky, so it is raised once per (function, size).

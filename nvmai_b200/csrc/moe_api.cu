@@ -34,10 +34,12 @@
 #include "persistent_batch.cuh"
 #include "persistent_decode.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.h"
 
 using namespace nvmai;
 
 static std::atomic<uint64_t> g_launches{0};
+void nvmai::count_launches(uint64_t launches) { g_launches.fetch_add(launches, std::memory_order_relaxed); }
 
 struct LayerViews {
     bool registered = false;
@@ -383,22 +385,6 @@ int launch_stage1(nvmai_cuda_moe *h, const LayerViews &lv, const XSource &xsrc, 
                                  dim3(grid), dim3(kDecodeThreads), smem, st, pdl, p);
         });
     });
-}
-
-// cuTensorMapEncodeTiled, looked up through the runtime (the library does not link libcuda)
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeTiledFn>(p);
-    }();
-    return fn;
 }
 
 // One tensor map: `rank` dimensions, dim 0 contiguous; strides in bytes for dims 1.. .

@@ -1,0 +1,409 @@
+// Rows sorted by expert and back, their gradients, and 8-bit codes of rows: kernels and entry points.
+#include "../../include/nvmai_cuda_moe.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "launch.h"
+#include "row_elem.cuh"
+#include "tma.cuh"
+
+using namespace nvmai;
+
+namespace {
+
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+
+// ---- sort_rows ------------------------------------------------------------------------------------------
+// A stable counting sort: the row of a pair is (kept pairs of smaller experts) + (pairs of its expert in front of it).  Each
+// block has a run of tokens; it counts the experts of all pairs, those in front of its run apart, and ranks its own pairs
+// with one warp, 32 at a time (__match_any_sync gives the pairs of the same expert).  Then its warps move the tokens' rows.
+constexpr int kSortThreads = 1024;
+constexpr uint32_t kSortBlocks = 148;
+
+struct SortParams {
+    const uint32_t *idx; uint32_t tokens, top_k, E;
+    uint32_t *position, *source, *begin;
+    const void *x; size_t x_stride; uint32_t d;
+    void *rows; size_t rows_stride;
+    float *row_scales;
+};
+
+// sum over the threads in front of this one (1024 threads); *total gets the sum over all
+__device__ __forceinline__ uint32_t block_exclusive_sum(uint32_t v, uint32_t *warp_sums, uint32_t *total) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= (uint32_t)o) s += up;
+    }
+    if (lane == 31u) warp_sums[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t w = warp_sums[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= (uint32_t)o) w += up;
+        }
+        warp_sums[lane] = w;
+    }
+    __syncthreads();
+    *total = warp_sums[31];
+    return s - v + (warp ? warp_sums[warp - 1] : 0u);
+}
+
+// MOVE: 0 the order alone, 1 rows as they are, 2 as codes.  T: what a row is read as (MOVE 1: bits of that size), V at a time.
+template <typename T, int V, int MOVE>
+__global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
+    __shared__ uint32_t before[kRowMaxExperts + 1], rest[kRowMaxExperts + 1], warp_sums[32];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t first = (uint32_t)((uint64_t)p.tokens * blockIdx.x / gridDim.x);
+    const uint32_t last = (uint32_t)((uint64_t)p.tokens * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t pairs = p.tokens * p.top_k, lo = first * p.top_k, hi = last * p.top_k;
+    for (uint32_t e = tid; e <= p.E; e += kSortThreads) before[e] = rest[e] = 0u;
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
+    for (uint32_t i = tid; i < pairs; i += kSortThreads) {
+        const uint32_t e = min(p.idx[i], p.E);
+        atomicAdd(i < lo ? &before[e] : &rest[e], 1u);
+    }
+    __syncthreads();
+    const uint32_t ahead = tid < p.E ? before[tid] : 0u;
+    uint32_t kept;
+    const uint32_t base = block_exclusive_sum(tid < p.E ? ahead + rest[tid] : 0u, warp_sums, &kept);
+    if (tid < p.E) {
+        before[tid] = base + ahead;              // row of the next pair of this expert
+        if (blockIdx.x == 0) p.begin[tid] = base;
+    }
+    if (tid == 0) {
+        before[p.E] += kept;                     // pairs that are not kept name the rows behind
+        if (blockIdx.x == 0) p.begin[p.E] = kept;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        for (uint32_t i0 = lo; i0 < hi; i0 += 32u) {
+            const uint32_t i = i0 + lane;
+            const uint32_t e = i < hi ? min(p.idx[i], p.E) : 0xFFFFFFFFu;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            uint32_t row = 0;
+            if (i < hi) row = before[e] + __popc(same & ((1u << lane) - 1u));
+            __syncwarp();
+            if (i < hi) {
+                if ((same >> lane) == 1u) before[e] = row + 1u;          // the last of them
+                p.source[row] = e < p.E ? i : kNoRow;
+                p.position[i] = e < p.E ? row : kNoRow;
+            }
+            __syncwarp();
+        }
+    }
+    if constexpr (MOVE != 0) {
+        __syncthreads();
+        // a warp takes a token's row, or a part of it where the block has fewer tokens than warps
+        const uint32_t mine = last - first, warps = kSortThreads / 32;
+        const uint32_t parts = mine == 0 || mine >= warps ? 1u : warps / mine;
+        const uint32_t pieces = p.d / V, each = (pieces + parts - 1u) / parts;
+        for (uint32_t u = warp; u < mine * parts; u += warps) {
+            const uint32_t t = first + u / parts, part = u % parts;
+            const uint32_t c0 = part * each, c1 = min(pieces, c0 + each);
+            const T *src = static_cast<const T *>(p.x) + (size_t)t * p.x_stride;
+            const uint32_t *pos = p.position + (size_t)t * p.top_k;
+            if constexpr (MOVE == 1) {
+                using P = Piece<T, V>;
+#pragma unroll 4
+                for (uint32_t c = c0 + lane; c < c1; c += 32u) {
+                    const P v = reinterpret_cast<const P *>(src)[c];
+                    for (uint32_t k = 0; k < p.top_k; ++k) {
+                        const uint32_t row = pos[k];
+                        if (row != kNoRow) reinterpret_cast<P *>(static_cast<T *>(p.rows) + (size_t)row * p.rows_stride)[c] = v;
+                    }
+                }
+            } else {
+                using P = Piece<T, V>;
+                using Q = Piece<int8_t, V>;
+                uint32_t m = 0;
+#pragma unroll 4
+                for (uint32_t c = lane; c < pieces; c += 32u) {
+                    const P v = reinterpret_cast<const P *>(src)[c];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) m = max(m, magnitude_bits(elem_to_float(v.v[i])));
+                }
+                m = __reduce_max_sync(0xffffffffu, m);
+                const RowScale rs = row_scale_bits(m);
+#pragma unroll 4
+                for (uint32_t c = c0 + lane; c < c1; c += 32u) {
+                    const P v = reinterpret_cast<const P *>(src)[c];
+                    Q q;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) q.v[i] = row_code(elem_to_float(v.v[i]), rs);
+                    for (uint32_t k = 0; k < p.top_k; ++k) {
+                        const uint32_t row = pos[k];
+                        if (row != kNoRow) reinterpret_cast<Q *>(static_cast<int8_t *>(p.rows) + (size_t)row * p.rows_stride)[c] = q;
+                    }
+                }
+                if (part == 0)
+                    for (uint32_t k = lane; k < p.top_k; k += 32u)
+                        if (pos[k] != kNoRow) p.row_scales[pos[k]] = rs.scale;
+            }
+        }
+    }
+}
+
+// ---- merge_rows -----------------------------------------------------------------------------------------
+struct MergeParams {
+    const void *rows; size_t rows_stride; uint32_t n_rows;
+    const uint32_t *position; const void *w; uint32_t w_elem;
+    uint32_t tokens, top_k, d;
+    const void *base; size_t base_stride;
+    void *y; size_t y_stride;
+};
+
+// A thread sums V neighbouring elements of one token over its slots.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
+    using P = Piece<T, V>;
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t t = blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= p.tokens) return;
+    const uint32_t *pos = p.position + (size_t)t * p.top_k;
+    for (uint32_t c = threadIdx.x; c < p.d / V; c += blockDim.x) {
+        float acc[V];
+        if (p.base != nullptr) {
+            const P b = reinterpret_cast<const P *>(static_cast<const T *>(p.base) + (size_t)t * p.base_stride)[c];
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = elem_to_float(b.v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+        }
+#pragma unroll 8
+        for (uint32_t k = 0; k < p.top_k; ++k) {
+            const uint32_t row = pos[k];
+            if (row >= p.n_rows) continue;
+            const float w = p.w != nullptr ? load_elem(p.w, p.w_elem, (size_t)t * p.top_k + k) : 1.0f;
+            const P v = reinterpret_cast<const P *>(static_cast<const T *>(p.rows) + (size_t)row * p.rows_stride)[c];
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, elem_to_float(v.v[i]), acc[i]);
+        }
+        P o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = elem_from_float<T>(acc[i]);
+        reinterpret_cast<P *>(static_cast<T *>(p.y) + (size_t)t * p.y_stride)[c] = o;
+    }
+}
+
+struct MergeGradParams {
+    const void *dy; size_t dy_stride;
+    const void *rows; size_t rows_stride; uint32_t n_rows;
+    const uint32_t *position; const void *w; uint32_t w_elem;
+    uint32_t pairs, top_k, d;
+    void *drows; size_t drows_stride;
+    float *dw;
+};
+
+// A warp per pair; the eight warps of a block share the rows of dy in the L1.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) merge_rows_grad_kernel(MergeGradParams p) {
+    using P = Piece<T, V>;
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t pair = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+    if (pair >= p.pairs) return;
+    const uint32_t row = p.position[pair];
+    if (row >= p.n_rows) {
+        if (p.dw != nullptr && lane == 0) p.dw[pair] = 0.0f;
+        return;
+    }
+    const float w = p.w != nullptr ? load_elem(p.w, p.w_elem, pair) : 1.0f;
+    const P *dy = reinterpret_cast<const P *>(static_cast<const T *>(p.dy) + (size_t)(pair / p.top_k) * p.dy_stride);
+    const P *v = reinterpret_cast<const P *>(static_cast<const T *>(p.rows) + (size_t)row * p.rows_stride);
+    P *o = reinterpret_cast<P *>(static_cast<T *>(p.drows) + (size_t)row * p.drows_stride);
+    float dot = 0.0f;
+#pragma unroll 4
+    for (uint32_t c = lane; c < p.d / V; c += 32u) {
+        const P g = dy[c];
+        if (p.dw != nullptr) {
+            const P r = v[c];
+#pragma unroll
+            for (int i = 0; i < V; ++i) dot = fmaf(elem_to_float(g.v[i]), elem_to_float(r.v[i]), dot);
+        }
+        if (p.drows != nullptr) {
+            P s;
+#pragma unroll
+            for (int i = 0; i < V; ++i) s.v[i] = elem_from_float<T>(w * elem_to_float(g.v[i]));
+            o[c] = s;
+        }
+    }
+    if (p.dw != nullptr) {
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+        if (lane == 0) p.dw[pair] = dot;
+    }
+}
+
+// ---- quantize_rows --------------------------------------------------------------------------------------
+struct QuantizeParams {
+    const void *x; size_t x_stride; uint32_t rows, n;
+    int8_t *q; size_t q_stride;
+    float *scales;
+};
+
+// A warp per row: the largest magnitude, then the codes (the row comes from the L1 the second time).
+template <typename T, int V>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p) {
+    using P = Piece<T, V>;
+    using Q = Piece<int8_t, V>;
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t row = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+    if (row >= p.rows) return;
+    const P *src = reinterpret_cast<const P *>(static_cast<const T *>(p.x) + (size_t)row * p.x_stride);
+    Q *dst = reinterpret_cast<Q *>(p.q + (size_t)row * p.q_stride);
+    uint32_t m = 0;
+#pragma unroll 4
+    for (uint32_t c = lane; c < p.n / V; c += 32u) {
+        const P v = src[c];
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = max(m, magnitude_bits(elem_to_float(v.v[i])));
+    }
+    const RowScale rs = row_scale_bits(__reduce_max_sync(0xffffffffu, m));
+#pragma unroll 4
+    for (uint32_t c = lane; c < p.n / V; c += 32u) {
+        const P v = src[c];
+        Q q;
+#pragma unroll
+        for (int i = 0; i < V; ++i) q.v[i] = row_code(elem_to_float(v.v[i]), rs);
+        dst[c] = q;
+    }
+    if (lane == 0) p.scales[row] = rs.scale;
+}
+
+// ---- launches -------------------------------------------------------------------------------------------
+
+int launched(cudaError_t e) {
+    count_launches(1);
+    if (e != cudaSuccess) cudaGetLastError();
+    return e == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
+}
+
+// Elements a thread moves at once: 16 bytes where every buffer starts on such a boundary, its rows are that far apart
+// and a row is a whole number of them; one element otherwise.
+struct Rows { const void *p; size_t stride, size; };
+template <typename F>
+auto with_pieces(uint32_t elem, uint32_t d, std::initializer_list<Rows> rows, F &&f) {
+    const size_t v = 16 / elem_size(elem);
+    bool wide = d % v == 0;
+    for (const Rows &r : rows)
+        if (r.p != nullptr) wide = wide && r.stride % v == 0 && aligned_to(r.p, std::min<size_t>(16, v * r.size));
+    using std::integral_constant;
+    if (elem == ELEM_F32) return wide ? f(float{}, integral_constant<int, 4>{}) : f(float{}, integral_constant<int, 1>{});
+    if (elem == ELEM_BF16) return wide ? f(__nv_bfloat16{}, integral_constant<int, 8>{}) : f(__nv_bfloat16{}, integral_constant<int, 1>{});
+    return wide ? f(__half{}, integral_constant<int, 8>{}) : f(__half{}, integral_constant<int, 1>{});
+}
+
+}  // namespace
+
+cudaError_t nvmai::launch_quantize(const void *x, uint32_t elem, uint32_t x_stride, uint32_t rows, uint32_t n, int8_t *q, uint32_t q_stride,
+                                   float *scales, cudaStream_t st) {
+    const QuantizeParams p{x, x_stride, rows, n, q, q_stride, scales};
+    return with_pieces(elem, n, {{x, x_stride, elem_size(elem)}, {q, q_stride, 1}}, [&](auto T, auto V) {
+        return launch_pdl(quantize_rows_kernel<decltype(T), decltype(V)::value>, dim3((rows + 7) / 8), dim3(256), 0, st, true, p);
+    });
+}
+
+extern "C" {
+
+uint64_t nvmai_cuda_moe_sort_rows_workspace(uint32_t, uint32_t, uint32_t) { return 0; }
+
+int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_k, uint32_t num_experts, uint32_t *position,
+                             uint32_t *source, uint32_t *expert_begin, const void *x, uint32_t x_elem, uint32_t x_stride, uint32_t d,
+                             void *rows, uint32_t rows_elem, uint32_t rows_stride, float *row_scales, void *workspace,
+                             uint64_t workspace_bytes, void *stream) {
+    if (!expert_begin || (tokens != 0 && (!idx || !position || !source))) return NVMAI_CUDA_EINVAL;
+    if (top_k == 0 || top_k > kRowMaxTopK || num_experts == 0 || num_experts > kRowMaxExperts) return NVMAI_CUDA_ERANGE;
+    if ((uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+    if (!aligned_to(idx, 4) || !aligned_to(position, 4) || !aligned_to(source, 4) || !aligned_to(expert_begin, 4)) return NVMAI_CUDA_EINVAL;
+    if ((x == nullptr) != (rows == nullptr)) return NVMAI_CUDA_EINVAL;
+    if (x != nullptr) {
+        if (x_elem > ELEM_BF16 || (rows_elem != x_elem && rows_elem != ELEM_I8)) return NVMAI_CUDA_EINVAL;
+        if (d == 0 || x_stride < d || rows_stride < d) return NVMAI_CUDA_EINVAL;
+        if (!aligned_to(x, elem_size(x_elem)) || !aligned_to(rows, elem_size(rows_elem))) return NVMAI_CUDA_EINVAL;
+        if ((rows_elem == ELEM_I8) != (row_scales != nullptr) || !aligned_to(row_scales, 4)) return NVMAI_CUDA_EINVAL;
+    }
+    if (workspace_bytes < nvmai_cuda_moe_sort_rows_workspace(tokens, top_k, num_experts)) return NVMAI_CUDA_ERANGE;
+    if (!on_current_device({idx, position, source, expert_begin, x, rows, row_scales})) return NVMAI_CUDA_EINVAL;
+    const SortParams p{idx, tokens, top_k, num_experts, position, source, expert_begin, x, x_stride, d, rows, rows_stride, row_scales};
+    const dim3 grid(std::max(1u, std::min(tokens, kSortBlocks))), block(kSortThreads);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (x == nullptr) return launched(launch_pdl(sort_rows_kernel<float, 1, 0>, grid, block, 0, st, true, p));
+    return with_pieces(x_elem, d, {{x, x_stride, elem_size(x_elem)}, {rows, rows_stride, elem_size(rows_elem)}}, [&](auto T, auto V) {
+        constexpr int v = decltype(V)::value;
+        if (rows_elem == ELEM_I8) return launched(launch_pdl(sort_rows_kernel<decltype(T), v, 2>, grid, block, 0, st, true, p));
+        return launched(launch_pdl(sort_rows_kernel<decltype(T), v, 1>, grid, block, 0, st, true, p));
+    });
+}
+
+int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_t rows_stride, uint32_t n_rows, const uint32_t *position,
+                              const void *w, uint32_t w_elem, uint32_t tokens, uint32_t top_k, uint32_t d, const void *base,
+                              uint32_t base_stride, void *y, uint32_t y_stride, void *stream) {
+    if ((n_rows != 0 && !rows) || (tokens != 0 && (!position || !y))) return NVMAI_CUDA_EINVAL;
+    if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
+    if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+    if (d == 0 || y_stride < d || (n_rows != 0 && rows_stride < d) || (base && base_stride < d)) return NVMAI_CUDA_EINVAL;
+    const size_t size = elem_size(elem);
+    if (!aligned_to(rows, size) || !aligned_to(y, size) || !aligned_to(base, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
+        !aligned_to(position, 4))
+        return NVMAI_CUDA_EINVAL;
+    if (tokens == 0) return NVMAI_CUDA_OK;
+    if (!on_current_device({n_rows != 0 ? rows : nullptr, position, w, base, y})) return NVMAI_CUDA_EINVAL;
+    const MergeParams p{rows, rows_stride, n_rows, position, w, w_elem, tokens, top_k, d, base, base_stride, y, y_stride};
+    return with_pieces(elem, d, {{n_rows != 0 ? rows : nullptr, rows_stride, size}, {base, base_stride, size}, {y, y_stride, size}}, [&](auto T, auto V) {
+        constexpr int v = decltype(V)::value;
+        uint32_t tx = 32;
+        while (tx < 256 && tx < d / v) tx *= 2;
+        const uint32_t ty = 256 / tx;
+        return launched(launch_pdl(merge_rows_kernel<decltype(T), v>, dim3((tokens + ty - 1) / ty), dim3(tx, ty), 0,
+                                   static_cast<cudaStream_t>(stream), true, p));
+    });
+}
+
+int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_stride, const void *rows, uint32_t rows_stride,
+                                   uint32_t n_rows, const uint32_t *position, const void *w, uint32_t w_elem, uint32_t tokens,
+                                   uint32_t top_k, uint32_t d, void *drows, uint32_t drows_stride, float *dw, void *stream) {
+    if ((!drows && !dw) || (tokens != 0 && (!dy || !position))) return NVMAI_CUDA_EINVAL;
+    if (dw && n_rows != 0 && !rows) return NVMAI_CUDA_EINVAL;
+    if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
+    if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+    if (d == 0 || dy_stride < d || (drows && drows_stride < d) || (dw && n_rows != 0 && rows_stride < d)) return NVMAI_CUDA_EINVAL;
+    const size_t size = elem_size(elem);
+    if (!aligned_to(dy, size) || !aligned_to(rows, size) || !aligned_to(drows, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
+        !aligned_to(dw, 4) || !aligned_to(position, 4))
+        return NVMAI_CUDA_EINVAL;
+    if (tokens == 0) return NVMAI_CUDA_OK;
+    const void *read = dw && n_rows != 0 ? rows : nullptr;       // the rows are read for dw alone
+    if (!on_current_device({dy, read, position, w, n_rows != 0 ? drows : nullptr, dw})) return NVMAI_CUDA_EINVAL;
+    const uint32_t pairs = tokens * top_k;
+    const MergeGradParams p{dy, dy_stride, rows, rows_stride, n_rows, position, w, w_elem, pairs, top_k, d, drows, drows_stride, dw};
+    return with_pieces(elem, d, {{dy, dy_stride, size}, {read, rows_stride, size}, {drows, drows_stride, size}}, [&](auto T, auto V) {
+        return launched(launch_pdl(merge_rows_grad_kernel<decltype(T), decltype(V)::value>, dim3((pairs + 7) / 8), dim3(256), 0,
+                                   static_cast<cudaStream_t>(stream), true, p));
+    });
+}
+
+int nvmai_cuda_moe_quantize_rows(const void *x, uint32_t elem, uint32_t x_stride, uint32_t rows, uint32_t n, void *q, uint32_t q_stride,
+                                 float *scales, void *stream) {
+    if (rows != 0 && (!x || !q || !scales)) return NVMAI_CUDA_EINVAL;
+    if (elem > ELEM_BF16 || n == 0 || x_stride < n || q_stride < n) return NVMAI_CUDA_EINVAL;
+    if (!aligned_to(x, elem_size(elem)) || !aligned_to(scales, 4)) return NVMAI_CUDA_EINVAL;
+    if (rows == 0) return NVMAI_CUDA_OK;
+    if (!on_current_device({x, q, scales})) return NVMAI_CUDA_EINVAL;
+    return launched(launch_quantize(x, elem, x_stride, rows, n, static_cast<int8_t *>(q), q_stride, scales,
+                                    static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,35 @@
+// Between the row operators' translation units: element types, checks of arguments, the quantisation launcher.
+#pragma once
+#include <cuda_runtime.h>
+#include <initializer_list>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace nvmai {
+
+enum : uint32_t { ELEM_F16 = 0, ELEM_F32 = 1, ELEM_BF16 = 2, ELEM_I8 = 3 };
+constexpr uint32_t kRowMaxExperts = 1024, kRowMaxTopK = 64;
+
+inline size_t elem_size(uint32_t e) { return e == ELEM_F32 ? 4 : e == ELEM_I8 ? 1 : 2; }
+inline bool aligned_to(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Every pointer given (null ones aside) is memory that the current device can read: a buffer of another device or of the
+// host would be an illegal address in the kernel.  An error is cleared: the call is refused, the context is as it was.
+inline bool on_current_device(std::initializer_list<const void *> ptrs) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return false; }
+    for (const void *p : ptrs) {
+        if (p == nullptr) continue;
+        cudaPointerAttributes a;
+        if (cudaPointerGetAttributes(&a, p) != cudaSuccess) { cudaGetLastError(); return false; }
+        if (a.type == cudaMemoryTypeUnregistered || a.devicePointer == nullptr) return false;
+        if (a.type == cudaMemoryTypeDevice && a.device != dev) return false;
+    }
+    return true;
+}
+
+// rows of `n` elements -> codes and scales; arguments checked by the caller
+cudaError_t launch_quantize(const void *x, uint32_t elem, uint32_t x_stride, uint32_t rows, uint32_t n, int8_t *q, uint32_t q_stride,
+                            float *scales, cudaStream_t st);
+
+}  // namespace nvmai

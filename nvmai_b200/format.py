@@ -12,7 +12,8 @@ import numpy as np
 
 GROUP = 64
 META_BF16, META_FP16 = 0, 1
-ACT_SILU, ACT_GELU_TANH = 0, 1
+ACT_SILU, ACT_GELU_TANH, ACT_NONE = 0, 1, 2
+ELEM_F16, ELEM_F32, ELEM_BF16, ELEM_I8 = 0, 1, 2, 3
 OUT_FP16, OUT_FP32 = 0, 1
 ROUTER_DENSE_F16, ROUTER_AFFINE4, ROUTER_AFFINE8 = 0, 4, 8
 GATE_NONE = 0xFFFFFFFF
