@@ -1,0 +1,273 @@
+// Products of many rows with matrices of 8-bit codes: tcgen05.mma kind::i8 (32-bit integer sums) from TMA-fed shared memory.
+//
+// The matrix is the M operand (128 channels a tile), the rows are N: a tile takes any multiple of 16 rows, so an expert with
+// few rows costs few columns.  Two tiles of channels share a block of rows (with an activation: the gate rows and the up rows
+// of the same 128 features, so that one thread has both accumulators of an output).  Persistent: one block per SM, units in
+// the order (expert, channel tile, row tile), so that the row tiles that read the same codes run beside each other and the
+// codes cross HBM once.  Warps: 8 epilogue, 1 for the copies, 1 for the MMAs; the accumulators are double-buffered.
+#pragma once
+#include "common.cuh"
+#include "row_elem.cuh"
+#include "tcgen05.cuh"
+
+namespace nvmai {
+
+constexpr int kIgEpilogueWarps = 8, kIgCopyWarp = 8, kIgMmaWarp = 9, kIgThreads = 320;
+constexpr uint32_t kIgMaxStages = 8, kIgBoxRows = 32;
+constexpr uint32_t kIgTileBytes = 128 * 128;           // 128 channels x 128 codes
+constexpr uint32_t kActNone = 2;
+
+struct IgParams {
+    uint32_t rows, k, n, channels, E;
+    const uint32_t *begin;               // first row of each expert, or nullptr: one matrix
+    const float *a_scales, *b_scales;
+    uint32_t act;
+    void *out; size_t out_stride;
+    uint32_t subs, nt, stages;           // channel tiles of a unit, most rows of a unit (a multiple of 32), ring slots
+    uint32_t channel_tiles;              // units across the channels
+    unsigned int *status;
+};
+struct alignas(64) IgArgs {
+    CUtensorMap a, b;                    // [rows][k], [E * channels][k] bytes; boxes of 32 and of 128 rows x 128 bytes
+    IgParams p;
+};
+
+__device__ __forceinline__ void umma_i8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor, kind::i8: 32-bit integer accumulator (2 in bits 4-5), A and B signed (1 in bits 7-9 and 10-12),
+// both K-major, N >> 3 in bits 17-22, M >> 4 in bits 24-28.
+__device__ __forceinline__ uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+struct IgShared {
+    uint64_t full[kIgMaxStages], empty[kIgMaxStages], acc_full[2], acc_empty[2], drained;
+    uint32_t tmem_slot, warp_sums[8];
+    uint32_t gave_up;
+    uint32_t tiles[kRowMaxExperts + 1];       // row tiles of the experts in front
+    uint32_t first[kRowMaxExperts + 1];       // first row of each expert
+};
+
+struct IgUnit { uint32_t e, row, count, ch; };       // rows row .. row + count - 1 of expert e, channel tile ch
+
+__device__ __forceinline__ IgUnit ig_unit(const IgShared &s, const IgParams &p, uint32_t u) {
+    uint32_t lo = 0, hi = p.E;                        // tiles[lo] * C <= u < tiles[hi] * C
+    const uint32_t tile = u / p.channel_tiles;        // a row tile of the same expert
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (s.tiles[mid] <= tile) lo = mid; else hi = mid;
+    }
+    const uint32_t t_e = s.tiles[lo + 1] - s.tiles[lo], r = u - s.tiles[lo] * p.channel_tiles;
+    const uint32_t n_e = s.first[lo + 1] - s.first[lo];
+    const uint32_t per = ((n_e + t_e - 1) / t_e + 15u) & ~15u;      // even tiles; the last one keeps at least a row
+    IgUnit un;
+    un.e = lo;
+    un.ch = r / t_e;
+    const uint32_t at = (r - un.ch * t_e) * per;
+    un.row = s.first[lo] + at;
+    un.count = min(per, n_e - at);
+    return un;
+}
+
+template <typename OUT, bool GATED>
+__global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_constant__ IgArgs args) {
+    const IgParams &p = args.p;
+    __shared__ IgShared s;
+    extern __shared__ unsigned char ig_ring_raw[];
+    const uint32_t ring = (smem_addr(ig_ring_raw) + 1023u) & ~1023u;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
+
+    if (tid == 0) {
+        for (uint32_t i = 0; i < p.stages; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
+        for (uint32_t i = 0; i < 2; ++i) { mbar_init(&s.acc_full[i], 1); mbar_init(&s.acc_empty[i], kIgEpilogueWarps); }
+        mbar_init(&s.drained, 1);
+        mbar_fence_init();
+        s.gave_up = 0u;
+    }
+    if (warp == kIgMmaWarp) {
+        tmem_alloc(&s.tmem_slot, 512);
+        tmem_relinquish();
+    }
+    if (warp == kIgCopyWarp && lane == 0) { tma_prefetch_map(&args.a); tma_prefetch_map(&args.b); }
+    pdl_wait();
+    pdl_launch_dependents();
+    // Row tiles in front of each expert: a thread adds up to four experts, the warps' sums are put together.  Begins behind
+    // the last row or out of order give an expert fewer rows or none, never rows outside.
+    {
+        const uint32_t per = (p.E + 255u) / 256u, e0 = tid * per;
+        uint32_t mine[4] = {0, 0, 0, 0}, sum = 0;
+        if (tid < 256u) {
+            for (uint32_t i = 0; i < per && e0 + i < p.E; ++i) {
+                const uint32_t a = p.begin ? min(p.begin[e0 + i], p.rows) : 0u, b = p.begin ? min(p.begin[e0 + i + 1], p.rows) : p.rows;
+                mine[i] = b > a ? (b - a + p.nt - 1u) / p.nt : 0u;
+                s.first[e0 + i] = a;
+                sum += mine[i];
+            }
+            uint32_t run = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= (uint32_t)o) run += up;
+            }
+            if (lane == 31u) s.warp_sums[warp] = run;
+            sum = run - sum;
+        }
+        if (tid == 0) s.first[p.E] = p.begin ? min(p.begin[p.E], p.rows) : p.rows;
+        tc_fence_before_sync();
+        __syncthreads();
+        tc_fence_after_sync();
+        if (tid < 256u) {
+            for (uint32_t w = 0; w < warp; ++w) sum += s.warp_sums[w];
+            for (uint32_t i = 0; i < per && e0 + i < p.E; ++i) {
+                s.tiles[e0 + i] = sum;
+                sum += mine[i];
+                if (e0 + i + 1 == p.E) s.tiles[p.E] = sum;
+            }
+        }
+        __syncthreads();
+    }
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s.tmem_slot);
+    const uint32_t total = s.tiles[p.E] * p.channel_tiles;
+    const uint32_t n_kb = (p.k + 127u) / 128u;
+    const uint32_t stage_bytes = p.subs * kIgTileBytes + p.nt * 128u;
+
+    // bounded by the GPU's nanosecond timer; a role that gives up tells the others
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait_short(bar, parity)) return true;
+        const unsigned long long t0 = global_timer_ns(), limit = g_wait_limit_ns;
+        for (;;) {
+#pragma unroll 1
+            for (int it = 0; it < 16; ++it)
+                if (mbar_try_wait_short(bar, parity)) return true;
+            if (*reinterpret_cast<volatile uint32_t *>(&s.gave_up) != 0u) return false;
+            if (global_timer_ns() - t0 > limit) break;
+        }
+        *reinterpret_cast<volatile uint32_t *>(&s.gave_up) = 1u;
+        atomicExch(p.status, 1u);
+        return false;
+    };
+
+    if (warp == kIgCopyWarp) {
+        if (elect_one()) {
+            uint32_t stage = 0, parity = 1, filled = 0;         // the first pass finds every slot empty
+            bool ok = true;
+            for (uint32_t u = blockIdx.x; ok && u < total; u += gridDim.x) {
+                const IgUnit un = ig_unit(s, p, u);
+                const uint32_t boxes = (un.count + kIgBoxRows - 1u) / kIgBoxRows;
+                const uint32_t bytes = p.subs * kIgTileBytes + boxes * kIgBoxRows * 128u;
+                const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : p.subs * 128u);
+                const uint32_t ch1 = GATED ? ch0 + p.n : ch0 + 128u;
+                for (uint32_t kb = 0; kb < n_kb; ++kb) {
+                    if (!(ok = wait(&s.empty[stage], parity))) break;
+                    const uint32_t slot = ring + stage * stage_bytes;
+                    mbar_expect_tx(&s.full[stage], bytes);
+                    tma_load_2d(slot, &args.b, kb * 128u, ch0, &s.full[stage]);
+                    if (p.subs == 2u) tma_load_2d(slot + kIgTileBytes, &args.b, kb * 128u, ch1, &s.full[stage]);
+                    for (uint32_t i = 0; i < boxes; ++i)
+                        tma_load_2d(slot + p.subs * kIgTileBytes + i * kIgBoxRows * 128u, &args.a, kb * 128u, un.row + i * kIgBoxRows, &s.full[stage]);
+                    ++filled;
+                    if (++stage == p.stages) { stage = 0; parity ^= 1u; }
+                }
+            }
+            if (!ok) {      // copies in flight end before the block does
+                const unsigned long long t0 = global_timer_ns();
+                for (uint32_t i = 0; i < min(filled, p.stages); ++i) {
+                    const uint32_t at = (stage + p.stages - 1u - i) % p.stages, lap = (filled - 1u - i) / p.stages;
+                    while (!mbar_try_wait_short(&s.full[at], lap & 1u) && global_timer_ns() - t0 < 1000000000ull) {}
+                }
+            }
+        }
+    } else if (warp == kIgMmaWarp) {
+        if (elect_one()) {
+            uint32_t stage = 0, parity = 0, it = 0;
+            bool ok = true;
+            for (uint32_t u = blockIdx.x; ok && u < total; u += gridDim.x, ++it) {
+                const IgUnit un = ig_unit(s, p, u);
+                const uint32_t idesc = umma_idesc_i8(128u, (un.count + 15u) & ~15u);
+                const uint32_t buf = it & 1u, acc = tmem + buf * p.subs * p.nt;
+                if (!(ok = wait(&s.acc_empty[buf], ((it >> 1) & 1u) ^ 1u))) break;
+                tc_fence_after_sync();
+                for (uint32_t kb = 0; kb < n_kb; ++kb) {
+                    if (!(ok = wait(&s.full[stage], parity))) break;
+                    tc_fence_after_sync();
+                    const uint32_t slot = ring + stage * stage_bytes;
+                    const uint64_t b = umma_desc_sw128(slot + p.subs * kIgTileBytes);
+                    for (uint32_t t = 0; t < p.subs; ++t) {
+                        const uint64_t a = umma_desc_sw128(slot + t * kIgTileBytes);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < 4u; ++kk)           // 32 codes = 32 bytes = 2 units of the descriptor's address
+                            umma_i8_ss(acc + t * p.nt, a + 2u * kk, b + 2u * kk, idesc, (kb | kk) != 0u ? 1u : 0u);
+                    }
+                    umma_commit(&s.empty[stage]);
+                    if (++stage == p.stages) { stage = 0; parity ^= 1u; }
+                }
+                if (ok) umma_commit(&s.acc_full[buf]);
+            }
+            if (!ok) {      // MMAs in flight end before their operands and accumulators go
+                umma_commit(&s.drained);
+                const unsigned long long t0 = global_timer_ns();
+                while (!mbar_try_wait_short(&s.drained, 0u) && global_timer_ns() - t0 < 1000000000ull) {}
+            }
+        }
+    } else {
+        const uint32_t quarter = warp & 3u, half = warp >> 2;
+        uint32_t it = 0;
+        for (uint32_t u = blockIdx.x; u < total; u += gridDim.x, ++it) {
+            const IgUnit un = ig_unit(s, p, u);
+            const uint32_t buf = it & 1u, acc = tmem + buf * p.subs * p.nt + ((quarter * 32u) << 16);
+            const uint32_t j0 = un.ch * (GATED ? 128u : p.subs * 128u) + quarter * 32u + lane;
+            const float *bs = p.b_scales + (size_t)un.e * p.channels;
+            float sb0 = 0.0f, sb1 = 0.0f;
+            if (j0 < p.n) sb0 = bs[j0];
+            if (GATED) { if (j0 < p.n) sb1 = bs[p.n + j0]; }
+            else if (p.subs == 2u && j0 + 128u < p.n) sb1 = bs[j0 + 128u];
+            if (!__all_sync(0xffffffffu, wait(&s.acc_full[buf], (it >> 1) & 1u))) break;
+            tc_fence_after_sync();
+            OUT *out = static_cast<OUT *>(p.out) + (size_t)un.row * p.out_stride + j0;
+            for (uint32_t c0 = half * 16u; c0 < un.count; c0 += 32u) {
+                const float sa_lane = c0 + (lane & 15u) < un.count ? p.a_scales[un.row + c0 + (lane & 15u)] : 0.0f;
+                uint32_t v0[16], v1[16];
+                tmem_ld16(acc + c0, v0);
+                if (p.subs == 2u) tmem_ld16(acc + p.nt + c0, v1);
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t c = 0; c < 16u; ++c) {
+                    const float sa = __shfl_sync(0xffffffffu, sa_lane, c);
+                    if (c0 + c >= un.count) continue;
+                    OUT *o = out + (size_t)(c0 + c) * p.out_stride;
+                    float x = (sa * sb0) * (float)(int)v0[c];
+                    if (GATED) {
+                        const float up = (sa * sb1) * (float)(int)v1[c];
+                        x = hidden_act(x, p.act) * up;
+                    } else if (p.subs == 2u && j0 + 128u < p.n) {
+                        o[128] = elem_from_float<OUT>((sa * sb1) * (float)(int)v1[c]);
+                    }
+                    if (j0 < p.n) o[0] = elem_from_float<OUT>(x);
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.acc_empty[buf]);
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == kIgMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace nvmai

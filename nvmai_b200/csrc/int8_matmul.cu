@@ -6,15 +6,17 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "int8_gemm.cuh"
 #include "launch.h"
 #include "row_elem.cuh"
+#include "tensor_map.h"
 #include "tma.cuh"
 
 using namespace nvmai;
 
 namespace {
 
-constexpr uint32_t kActNone = NVMAI_ACT_NONE;
+static_assert(kActNone == NVMAI_ACT_NONE && ACT_SILU == NVMAI_ACT_SILU && ACT_GELU == NVMAI_ACT_GELU_TANH, "activations of the header");
 
 struct MatmulParams {
     const int8_t *a; size_t a_stride; const float *a_scales;
@@ -82,6 +84,57 @@ size_t scales_offset(uint32_t rows, uint32_t k) { return ((size_t)rows * code_st
 
 static __device__ unsigned int g_int8_status;      // a bounded wait gave up (nvmai_cuda_moe_int8_matmul_status)
 
+// One tensor map of rows of codes in boxes of `box_rows` rows x 128 bytes, 128-byte swizzle; bytes outside read as zeros.
+bool code_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t k, uint64_t stride, uint32_t box_rows) {
+    const EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return false;
+    const cuuint64_t dim[2] = {k, rows}, str[1] = {stride};
+    const cuuint32_t box[2] = {128, box_rows}, one[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dim, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+unsigned int *status_word() {
+    static unsigned int *at[64] = {};
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (at[dev] == nullptr) {
+        void *p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_int8_status) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+        at[dev] = static_cast<unsigned int *>(p);
+    }
+    return at[dev];
+}
+
+constexpr uint32_t kSms = 148;
+
+cudaError_t launch_gemm(const MatmulParams &m, cudaStream_t st) {
+    IgArgs args;
+    IgParams &p = args.p;
+    p = IgParams{};
+    const bool gated = m.act != kActNone;
+    p.rows = m.rows; p.k = m.k; p.n = m.n; p.channels = m.channels; p.E = m.E; p.begin = m.begin;
+    p.a_scales = m.a_scales; p.b_scales = m.b_scales; p.act = m.act; p.out = m.out; p.out_stride = m.out_stride;
+    p.status = status_word();
+    if (!p.status || !code_map(&args.a, m.a, m.rows, m.k, m.a_stride, kIgBoxRows) ||
+        !code_map(&args.b, m.b, (uint64_t)m.E * m.channels, m.k, m.b_stride, 128)) return cudaErrorInvalidValue;
+    const uint32_t average = (m.rows + m.E - 1) / m.E;
+    p.nt = std::min(128u, std::max(32u, (average + 31) / 32 * 32));
+    p.subs = gated || (uint64_t)((m.n + 255) / 256) * ((m.rows + p.nt - 1) / p.nt) >= kSms ? 2 : 1;
+    p.channel_tiles = (m.n + (gated ? 128 : p.subs * 128) - 1) / (gated ? 128 : p.subs * 128);
+    const size_t stage = p.subs * kIgTileBytes + (size_t)p.nt * 128;
+    p.stages = (uint32_t)std::min<size_t>(kIgMaxStages, (227 * 1024 - sizeof(IgShared) - 2048) / stage);
+    const size_t smem = 1024 + p.stages * stage;
+    // units: at most a row tile for each expert that has rows and one for each nt rows
+    const uint64_t tiles = m.begin ? std::min<uint64_t>(m.rows, (uint64_t)m.E + m.rows / p.nt) : (m.rows + p.nt - 1) / p.nt;
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(kSms, tiles * p.channel_tiles);
+    auto go = [&](auto T) {
+        if (gated) return launch_pdl(int8_gemm_kernel<decltype(T), true>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
+        return launch_pdl(int8_gemm_kernel<decltype(T), false>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
+    };
+    return m.out_elem == ELEM_F16 ? go(__half{}) : m.out_elem == ELEM_BF16 ? go(__nv_bfloat16{}) : go(float{});
+}
+
 }  // namespace
 
 extern "C" {
@@ -127,7 +180,7 @@ int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride
         if (e != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
         p.a = q; p.a_stride = code_stride(k); p.a_scales = scales;
     }
-    const cudaError_t e = launch_pdl(int8_matmul_kernel, dim3(rows, (n + 7) / 8), dim3(256), 0, st, true, p);
+    const cudaError_t e = rows > 8 ? launch_gemm(p, st) : launch_pdl(int8_matmul_kernel, dim3(rows, (n + 7) / 8), dim3(256), 0, st, true, p);
     count_launches(1);
     if (e != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
     return NVMAI_CUDA_OK;
