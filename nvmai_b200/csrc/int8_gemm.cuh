@@ -4,7 +4,8 @@
 // few rows costs few columns.  Two tiles of channels share a block of rows (with an activation: the gate rows and the up rows
 // of the same 128 features, so that one thread has both accumulators of an output).  Persistent: one block per SM, units in
 // the order (expert, channel tile, row tile), so that the row tiles that read the same codes run beside each other and the
-// codes cross HBM once.  Warps: 8 epilogue, 1 for the copies, 1 for the MMAs; the accumulators are double-buffered.
+// codes cross HBM once.  Warps: 16 epilogue, 1 for the copies, 1 for the MMAs; the accumulators are
+// double-buffered where two sets fit.
 #pragma once
 #include "common.cuh"
 #include "row_elem.cuh"
@@ -12,7 +13,7 @@
 
 namespace nvmai {
 
-constexpr int kIgEpilogueWarps = 8, kIgCopyWarp = 8, kIgMmaWarp = 9, kIgThreads = 320;
+constexpr int kIgEpilogueWarps = 16, kIgCopyWarp = 16, kIgMmaWarp = 17, kIgThreads = 576;
 constexpr uint32_t kIgMaxStages = 8, kIgBoxRows = 32;
 constexpr uint32_t kIgTileBytes = 128 * 128;           // 128 channels x 128 codes
 constexpr uint32_t kActNone = 2;
@@ -23,7 +24,9 @@ struct IgParams {
     const float *a_scales, *b_scales;
     uint32_t act;
     void *out; size_t out_stride;
-    uint32_t subs, nt, stages;           // channel tiles of a unit, most rows of a unit (a multiple of 32), ring slots
+    uint32_t nt, stages;                 // most rows of a unit (a multiple of 32), ring slots
+    uint32_t accs;                       // sets of accumulators (2, or 1 where two do not fit)
+    uint32_t paired;                     // 16-bit outputs: two neighbouring channels go out in one store
     uint32_t channel_tiles;              // units across the channels
     unsigned int *status;
 };
@@ -53,12 +56,36 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr));
 }
 
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+// The gate's activation.  HALF, for 16-bit outputs: SiLU through the hardware's exp2 and reciprocal, whose error of (2 |g| + 8) 2^-24
+// (the argument's rounding, 2 ulp and 1 ulp) is below a hundredth of the output's rounding up to |g| = 80, past which SiLU
+// is below 1e-33 on the one side and g on the other.  The exact division costs more than the rest of an output.
+template <bool HALF>
+__device__ __forceinline__ float gate_act(float g, uint32_t act) {
+    if (HALF && act == ACT_SILU) {
+        float e, r;
+        asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+        return g * r;
+    }
+    return hidden_act(g, act);
+}
+
 struct IgShared {
     uint64_t full[kIgMaxStages], empty[kIgMaxStages], acc_full[2], acc_empty[2], drained;
     uint32_t tmem_slot, warp_sums[8];
     uint32_t gave_up;
     uint32_t tiles[kRowMaxExperts + 1];       // row tiles of the experts in front
     uint32_t first[kRowMaxExperts + 1];       // first row of each expert
+    float4 row_scales[kIgEpilogueWarps][16];  // of the columns of an epilogue warp
 };
 
 struct IgUnit { uint32_t e, row, count, ch; };       // rows row .. row + count - 1 of expert e, channel tile ch
@@ -82,7 +109,8 @@ __device__ __forceinline__ IgUnit ig_unit(const IgShared &s, const IgParams &p, 
     return un;
 }
 
-template <typename OUT, bool GATED>
+// SUBS: channel tiles of a unit (2 with an activation).
+template <typename OUT, bool GATED, uint32_t SUBS>
 __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_constant__ IgArgs args) {
     const IgParams &p = args.p;
     __shared__ IgShared s;
@@ -142,7 +170,7 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s.tmem_slot);
     const uint32_t total = s.tiles[p.E] * p.channel_tiles;
     const uint32_t n_kb = (p.k + 127u) / 128u;
-    const uint32_t stage_bytes = p.subs * kIgTileBytes + p.nt * 128u;
+    const uint32_t stage_bytes = SUBS * kIgTileBytes + p.nt * 128u;
 
     // bounded by the GPU's nanosecond timer; a role that gives up tells the others
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -167,17 +195,17 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
             for (uint32_t u = blockIdx.x; ok && u < total; u += gridDim.x) {
                 const IgUnit un = ig_unit(s, p, u);
                 const uint32_t boxes = (un.count + kIgBoxRows - 1u) / kIgBoxRows;
-                const uint32_t bytes = p.subs * kIgTileBytes + boxes * kIgBoxRows * 128u;
-                const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : p.subs * 128u);
+                const uint32_t bytes = SUBS * kIgTileBytes + boxes * kIgBoxRows * 128u;
+                const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : SUBS * 128u);
                 const uint32_t ch1 = GATED ? ch0 + p.n : ch0 + 128u;
                 for (uint32_t kb = 0; kb < n_kb; ++kb) {
                     if (!(ok = wait(&s.empty[stage], parity))) break;
                     const uint32_t slot = ring + stage * stage_bytes;
                     mbar_expect_tx(&s.full[stage], bytes);
                     tma_load_2d(slot, &args.b, kb * 128u, ch0, &s.full[stage]);
-                    if (p.subs == 2u) tma_load_2d(slot + kIgTileBytes, &args.b, kb * 128u, ch1, &s.full[stage]);
+                    if (SUBS == 2) tma_load_2d(slot + kIgTileBytes, &args.b, kb * 128u, ch1, &s.full[stage]);
                     for (uint32_t i = 0; i < boxes; ++i)
-                        tma_load_2d(slot + p.subs * kIgTileBytes + i * kIgBoxRows * 128u, &args.a, kb * 128u, un.row + i * kIgBoxRows, &s.full[stage]);
+                        tma_load_2d(slot + SUBS * kIgTileBytes + i * kIgBoxRows * 128u, &args.a, kb * 128u, un.row + i * kIgBoxRows, &s.full[stage]);
                     ++filled;
                     if (++stage == p.stages) { stage = 0; parity ^= 1u; }
                 }
@@ -193,23 +221,23 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
     } else if (warp == kIgMmaWarp) {
         if (elect_one()) {
             uint32_t stage = 0, parity = 0, it = 0;
+            const uint64_t ring_desc = umma_desc_sw128(ring);
             bool ok = true;
             for (uint32_t u = blockIdx.x; ok && u < total; u += gridDim.x, ++it) {
                 const IgUnit un = ig_unit(s, p, u);
                 const uint32_t idesc = umma_idesc_i8(128u, (un.count + 15u) & ~15u);
-                const uint32_t buf = it & 1u, acc = tmem + buf * p.subs * p.nt;
-                if (!(ok = wait(&s.acc_empty[buf], ((it >> 1) & 1u) ^ 1u))) break;
+                const uint32_t buf = p.accs == 2u ? it & 1u : 0u, turn = p.accs == 2u ? it >> 1 : it, acc = tmem + buf * SUBS * p.nt;
+                if (!(ok = wait(&s.acc_empty[buf], (turn & 1u) ^ 1u))) break;
                 tc_fence_after_sync();
                 for (uint32_t kb = 0; kb < n_kb; ++kb) {
                     if (!(ok = wait(&s.full[stage], parity))) break;
                     tc_fence_after_sync();
-                    const uint32_t slot = ring + stage * stage_bytes;
-                    const uint64_t b = umma_desc_sw128(slot + p.subs * kIgTileBytes);
-                    for (uint32_t t = 0; t < p.subs; ++t) {
-                        const uint64_t a = umma_desc_sw128(slot + t * kIgTileBytes);
+                    const uint64_t a = ring_desc + stage * (stage_bytes >> 4), b = a + (SUBS * kIgTileBytes >> 4);
+#pragma unroll
+                    for (uint32_t t = 0; t < SUBS; ++t) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < 4u; ++kk)           // 32 codes = 32 bytes = 2 units of the descriptor's address
-                            umma_i8_ss(acc + t * p.nt, a + 2u * kk, b + 2u * kk, idesc, (kb | kk) != 0u ? 1u : 0u);
+                            umma_i8_ss(acc + t * p.nt, a + t * (kIgTileBytes >> 4) + 2u * kk, b + 2u * kk, idesc, kk ? 1u : kb);
                     }
                     umma_commit(&s.empty[stage]);
                     if (++stage == p.stages) { stage = 0; parity ^= 1u; }
@@ -223,39 +251,74 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
             }
         }
     } else {
-        const uint32_t quarter = warp & 3u, half = warp >> 2;
+        // A warp has a quarter of the channels and every fourth run of 16 rows.  A lane has a channel, so two lanes exchange
+        // halves of two rows' values and each stores both channels of one row: half the stores.
+        constexpr bool kHalf = sizeof(OUT) == 2;
+        const uint32_t quarter = warp & 3u, part = warp >> 2, odd = lane & 1u;
+        const bool paired = kHalf && p.paired != 0u;
+        float4 *scales = s.row_scales[warp];
         uint32_t it = 0;
         for (uint32_t u = blockIdx.x; u < total; u += gridDim.x, ++it) {
             const IgUnit un = ig_unit(s, p, u);
-            const uint32_t buf = it & 1u, acc = tmem + buf * p.subs * p.nt + ((quarter * 32u) << 16);
-            const uint32_t j0 = un.ch * (GATED ? 128u : p.subs * 128u) + quarter * 32u + lane;
-            const float *bs = p.b_scales + (size_t)un.e * p.channels;
-            float sb0 = 0.0f, sb1 = 0.0f;
-            if (j0 < p.n) sb0 = bs[j0];
-            if (GATED) { if (j0 < p.n) sb1 = bs[p.n + j0]; }
-            else if (p.subs == 2u && j0 + 128u < p.n) sb1 = bs[j0 + 128u];
-            if (!__all_sync(0xffffffffu, wait(&s.acc_full[buf], (it >> 1) & 1u))) break;
-            tc_fence_after_sync();
-            OUT *out = static_cast<OUT *>(p.out) + (size_t)un.row * p.out_stride + j0;
-            for (uint32_t c0 = half * 16u; c0 < un.count; c0 += 32u) {
-                const float sa_lane = c0 + (lane & 15u) < un.count ? p.a_scales[un.row + c0 + (lane & 15u)] : 0.0f;
-                uint32_t v0[16], v1[16];
-                tmem_ld16(acc + c0, v0);
-                if (p.subs == 2u) tmem_ld16(acc + p.nt + c0, v1);
-                tmem_ld_wait();
+            const uint32_t buf = p.accs == 2u ? it & 1u : 0u, turn = p.accs == 2u ? it >> 1 : it;
+            const uint32_t acc = tmem + buf * SUBS * p.nt + ((quarter * 32u) << 16);
+            const uint32_t j0 = un.ch * (GATED ? 128u : SUBS * 128u) + quarter * 32u + lane;
+            const bool live0 = j0 < p.n, live1 = !GATED && SUBS == 2 && j0 + 128u < p.n;
+            const float *bs = p.b_scales + (size_t)un.e * p.channels + j0;
+            const float sb0 = live0 ? bs[0] : 0.0f, sb1 = GATED ? (live0 ? bs[p.n] : 0.0f) : (live1 ? bs[128] : 0.0f);
 #pragma unroll
-                for (uint32_t c = 0; c < 16u; ++c) {
-                    const float sa = __shfl_sync(0xffffffffu, sa_lane, c);
-                    if (c0 + c >= un.count) continue;
-                    OUT *o = out + (size_t)(c0 + c) * p.out_stride;
-                    float x = (sa * sb0) * (float)(int)v0[c];
-                    if (GATED) {
-                        const float up = (sa * sb1) * (float)(int)v1[c];
-                        x = hidden_act(x, p.act) * up;
-                    } else if (p.subs == 2u && j0 + 128u < p.n) {
-                        o[128] = elem_from_float<OUT>((sa * sb1) * (float)(int)v1[c]);
+            for (uint32_t i = 0; i < 2u; ++i) {                   // runs 2 i and 2 i + 1 of this warp
+                const uint32_t run = 2u * i + (lane >> 4), c = (part + 4u * run) * 16u + (lane & 15u);
+                reinterpret_cast<float *>(scales)[run * 16u + (lane & 15u)] = c < un.count ? p.a_scales[un.row + c] : 0.0f;
+            }
+            __syncwarp();
+            if (!__all_sync(0xffffffffu, wait(&s.acc_full[buf], turn & 1u))) break;
+            tc_fence_after_sync();
+            auto store = [&](const float (&x)[16], OUT *o, uint32_t live, bool mine) {
+                if constexpr (kHalf) {
+                    if (paired) {
+                        const uint32_t pick = odd ? 0x3276u : 0x5410u;
+                        o += odd ? p.out_stride - 1 : 0;
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; ++c, o += 2 * p.out_stride) {
+                            const uint32_t own = pack2<OUT>(x[2 * c], x[2 * c + 1]);
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+                            if (mine && 2u * c + odd < live) *reinterpret_cast<uint32_t *>(o) = __byte_perm(own, other, pick);
+                        }
+                        return;
                     }
-                    if (j0 < p.n) o[0] = elem_from_float<OUT>(x);
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < 16u; ++c, o += p.out_stride)
+                    if (mine && c < live) *o = elem_from_float<OUT>(x[c]);
+            };
+            for (uint32_t i = 0, c0 = part * 16u; c0 < un.count; ++i, c0 += 64u) {
+                OUT *out = static_cast<OUT *>(p.out) + (size_t)(un.row + c0) * p.out_stride + j0;
+                const uint32_t live = un.count - c0;
+                float x[16];
+                uint32_t v[16];
+                if constexpr (GATED) {
+                    uint32_t v1[16];
+                    tmem_ld16(acc + c0, v);
+                    tmem_ld16(acc + p.nt + c0, v1);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t c = 0; c < 16u; ++c) {
+                        const float sa = reinterpret_cast<const float *>(scales)[i * 16u + c];
+                        x[c] = gate_act<kHalf>((sa * sb0) * (float)(int)v[c], p.act) * ((sa * sb1) * (float)(int)v1[c]);
+                    }
+                    store(x, out, live, live0);
+                } else {
+#pragma unroll
+                    for (uint32_t t = 0; t < SUBS; ++t) {
+                        tmem_ld16(acc + t * p.nt + c0, v);
+                        tmem_ld_wait();
+                        const float sb = t ? sb1 : sb0;
+#pragma unroll
+                        for (uint32_t c = 0; c < 16u; ++c)
+                            x[c] = (reinterpret_cast<const float *>(scales)[i * 16u + c] * sb) * (float)(int)v[c];
+                        store(x, out + 128u * t, live, t ? live1 : live0);
+                    }
                 }
             }
             tc_fence_before_sync();

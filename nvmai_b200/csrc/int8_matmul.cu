@@ -4,9 +4,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "int8_gemm.cuh"
+#include "int8_stream.cuh"
 #include "launch.h"
 #include "row_elem.cuh"
 #include "tensor_map.h"
@@ -18,8 +21,8 @@ namespace {
 
 static_assert(kActNone == NVMAI_ACT_NONE && ACT_SILU == NVMAI_ACT_SILU && ACT_GELU == NVMAI_ACT_GELU_TANH, "activations of the header");
 
-struct MatmulParams {
-    const int8_t *a; size_t a_stride; const float *a_scales;
+struct Matmul {
+    const void *a; uint32_t a_elem; size_t a_stride; const float *a_scales;
     uint32_t rows, k;
     const int8_t *b; size_t b_stride; const float *b_scales;
     uint32_t n, channels, E;
@@ -27,56 +30,6 @@ struct MatmulParams {
     uint32_t act;
     void *out; uint32_t out_elem; size_t out_stride;
 };
-
-// The expert of a row: the last e with begin[e] <= row; E where the row is nobody's.
-__device__ __forceinline__ uint32_t expert_of_row(const uint32_t *begin, uint32_t E, uint32_t row) {
-    if (begin == nullptr) return 0;
-    if (row < begin[0] || row >= begin[E]) return E;
-    uint32_t lo = 0, hi = E;                     // begin[lo] <= row < begin[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (begin[mid] <= row) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-__device__ __forceinline__ void store_elem(void *out, uint32_t elem, size_t i, float v) {
-    if (elem == ELEM_F16) static_cast<__half *>(out)[i] = __float2half_rn(v);
-    else if (elem == ELEM_BF16) static_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(v);
-    else static_cast<float *>(out)[i] = v;
-}
-
-// sum over a row's codes, by one warp
-__device__ __forceinline__ int warp_dot(const int8_t *a, const int8_t *b, uint32_t k) {
-    const uint32_t lane = threadIdx.x & 31u;
-    int acc = 0;
-    const uint32_t whole = k & ~15u;
-    for (uint32_t i = lane * 16u; i < whole; i += 512u) {
-        const int4 x = *reinterpret_cast<const int4 *>(a + i), y = *reinterpret_cast<const int4 *>(b + i);
-        acc = __dp4a(x.x, y.x, acc); acc = __dp4a(x.y, y.y, acc);
-        acc = __dp4a(x.z, y.z, acc); acc = __dp4a(x.w, y.w, acc);
-    }
-    if (lane < (k & 15u)) acc += (int)a[whole + lane] * (int)b[whole + lane];
-    return __reduce_add_sync(0xffffffffu, acc);
-}
-
-// One warp per output.
-__global__ void __launch_bounds__(256) int8_matmul_kernel(MatmulParams p) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const uint32_t j = blockIdx.y * 8u + (threadIdx.x >> 5), r = blockIdx.x;
-    const uint32_t e = expert_of_row(p.begin, p.E, r);
-    if (j >= p.n || e >= p.E) return;
-    const int8_t *a = p.a + (size_t)r * p.a_stride;
-    const size_t ch = (size_t)e * p.channels + j;
-    const float sa = p.a_scales[r];
-    float v = (sa * p.b_scales[ch]) * (float)warp_dot(a, p.b + ch * p.b_stride, p.k);
-    if (p.act != kActNone) {
-        const float u = (sa * p.b_scales[ch + p.n]) * (float)warp_dot(a, p.b + (ch + p.n) * p.b_stride, p.k);
-        v = hidden_act(v, p.act) * u;
-    }
-    if ((threadIdx.x & 31u) == 0) store_elem(p.out, p.out_elem, (size_t)r * p.out_stride + j, v);
-}
 
 // codes and scales of rows that come as 16- or 32-bit elements
 size_t code_stride(uint32_t k) { return ((size_t)k + 15) & ~(size_t)15; }
@@ -108,7 +61,42 @@ unsigned int *status_word() {
 
 constexpr uint32_t kSms = 148;
 
-cudaError_t launch_gemm(const MatmulParams &m, cudaStream_t st) {
+struct IgTile { uint32_t subs, nt; };
+
+// Rows of a unit where the rows are spread over experts.  An expert's codes come once for each of its units (past the first from
+// the L2), so a unit holds the average expert and 2.5 times the spread of an even routing around it.  Past 128 rows
+// that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 115.5 us, 160 111.2,
+// 192 118.4 (three ring slots instead of four); 512 -> 2048: 75.7, 68.1, 71.1.  Two channel tiles a unit read the rows half
+// as often: 201 tokens down 50.6 us with one, 46.9 with two.
+IgTile grouped_tile(const Matmul &m) {
+    const float average = (float)m.rows / (float)m.E;
+    const uint32_t want = (uint32_t)std::ceil((average + 2.5f * std::sqrt(average)) / 32.0f) * 32u;
+    return IgTile{m.act != kActNone || m.n > 128 ? 2u : 1u, std::min(160u, std::max(32u, want))};
+}
+
+// One matrix: the cheapest tile by a model of the time, in ns, fitted to 16 shapes (40 to 16384 rows, 512 to 2048 codes, 300 to 2048
+// channels): a K block costs 104 and 4.1 for each KB of it, the last epilogue of a block 10 for each row and tile of its unit (an
+// activation counts double), earlier ones 6.5 beside the next unit or, with one set of accumulators, 10 in its way.  The
+// tile it picks took at most 7 % longer than the best one in those shapes; always 2 x 128 took up to 45 % longer.
+IgTile dense_tile(const Matmul &m) {
+    const bool gated = m.act != kActNone;
+    const float blocks = (float)((m.k + 127) / 128);
+    IgTile best{};
+    float best_ns = INFINITY;
+    for (uint32_t subs = gated ? 2 : 1; subs <= 2; ++subs)
+        for (uint32_t nt = 32; nt * subs <= 512 && nt <= 256; nt += 32) {
+            const uint64_t tiles = (m.rows + nt - 1) / nt, units = tiles * ((m.n + (gated ? 128 : 128 * subs) - 1) / (gated ? 128 : 128 * subs));
+            const float waves = (float)((units + kSms - 1) / kSms), per = (float)(((m.rows + tiles - 1) / tiles + 15) / 16 * 16);
+            const float kb = (float)(16 * subs) + std::ceil(per / 32.0f) * 4.0f, outs = per * (float)(subs * (gated ? 2 : 1));
+            const float epilogues = 2 * subs * nt <= 512 ? 10.4f + 6.5f * (waves - 1.0f) : 10.4f * waves;
+            const float ns = waves * blocks * (104.0f + 4.1f * kb) + outs * epilogues;
+            if (ns < best_ns) { best_ns = ns; best = IgTile{subs, nt}; }
+            if (nt >= m.rows) break;
+        }
+    return best;
+}
+
+cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     IgArgs args;
     IgParams &p = args.p;
     p = IgParams{};
@@ -118,21 +106,56 @@ cudaError_t launch_gemm(const MatmulParams &m, cudaStream_t st) {
     p.status = status_word();
     if (!p.status || !code_map(&args.a, m.a, m.rows, m.k, m.a_stride, kIgBoxRows) ||
         !code_map(&args.b, m.b, (uint64_t)m.E * m.channels, m.k, m.b_stride, 128)) return cudaErrorInvalidValue;
-    const uint32_t average = (m.rows + m.E - 1) / m.E;
-    p.nt = std::min(128u, std::max(32u, (average + 31) / 32 * 32));
-    p.subs = gated || (uint64_t)((m.n + 255) / 256) * ((m.rows + p.nt - 1) / p.nt) >= kSms ? 2 : 1;
-    p.channel_tiles = (m.n + (gated ? 128 : p.subs * 128) - 1) / (gated ? 128 : p.subs * 128);
-    const size_t stage = p.subs * kIgTileBytes + (size_t)p.nt * 128;
+    const IgTile tile = m.begin != nullptr ? grouped_tile(m) : dense_tile(m);
+    const uint32_t subs = tile.subs;
+    p.nt = tile.nt;
+    p.channel_tiles = (m.n + (gated ? 128 : subs * 128) - 1) / (gated ? 128 : subs * 128);
+    const size_t stage = subs * kIgTileBytes + (size_t)p.nt * 128;
+    p.accs = 2 * subs * p.nt <= 512 ? 2 : 1;
+    p.paired = m.n % 2 == 0 && m.out_stride % 2 == 0 && aligned_to(m.out, 4);
     p.stages = (uint32_t)std::min<size_t>(kIgMaxStages, (227 * 1024 - sizeof(IgShared) - 2048) / stage);
     const size_t smem = 1024 + p.stages * stage;
     // units: at most a row tile for each expert that has rows and one for each nt rows
     const uint64_t tiles = m.begin ? std::min<uint64_t>(m.rows, (uint64_t)m.E + m.rows / p.nt) : (m.rows + p.nt - 1) / p.nt;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>(kSms, tiles * p.channel_tiles);
     auto go = [&](auto T) {
-        if (gated) return launch_pdl(int8_gemm_kernel<decltype(T), true>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
-        return launch_pdl(int8_gemm_kernel<decltype(T), false>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
+        if (gated) return launch_pdl(int8_gemm_kernel<decltype(T), true, 2>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
+        if (subs == 2) return launch_pdl(int8_gemm_kernel<decltype(T), false, 2>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
+        return launch_pdl(int8_gemm_kernel<decltype(T), false, 1>, dim3(blocks), dim3(kIgThreads), smem, st, true, args);
     };
     return m.out_elem == ELEM_F16 ? go(__half{}) : m.out_elem == ELEM_BF16 ? go(__nv_bfloat16{}) : go(float{});
+}
+
+// Rows that the streaming kernel takes: its blocks go through the codes once for every 8 to 32 rows.
+uint32_t stream_tiles(const Matmul &m) {
+    const uint32_t nt = m.begin != nullptr || m.rows <= 8 ? 1 : m.rows <= 16 ? 2 : 4;
+    if (m.rows > (m.begin != nullptr ? 64u : 32u)) return 0;
+    return is_smem(m.k, nt) <= 200 * 1024 ? nt : 0;
+}
+
+cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
+    using std::integral_constant;
+    const bool gated = m.act != kActNone;
+    const IsParams p{m.a, m.a_stride, m.a_scales, m.rows, m.k, m.b, m.b_stride, m.b_scales, m.n, m.channels, m.E, m.begin, m.act,
+                     m.out, m.out_elem, m.out_stride, is_row_bytes(m.k)};
+    const dim3 grid((m.n + (gated ? 7 : 15)) / (gated ? 8 : 16), m.begin != nullptr ? m.rows : (m.rows + 8 * nt - 1) / (8 * nt));
+    auto go = [&](auto T, auto V, auto G, auto N) {
+        return launch_pdl(int8_stream_kernel<decltype(T), decltype(V)::value, decltype(G)::value, decltype(N)::value>, grid,
+                          dim3(kIsThreads), is_smem(m.k, nt), st, true, p);
+    };
+    auto with_tiles = [&](auto T, auto V, auto G) {
+        return nt == 1 ? go(T, V, G, integral_constant<int, 1>{}) : nt == 2 ? go(T, V, G, integral_constant<int, 2>{})
+                                                                           : go(T, V, G, integral_constant<int, 4>{});
+    };
+    auto with_gate = [&](auto T, auto V) {
+        return gated ? with_tiles(T, V, integral_constant<bool, true>{}) : with_tiles(T, V, integral_constant<bool, false>{});
+    };
+    if (m.a_elem == ELEM_I8) return with_gate(int8_t{}, integral_constant<int, 16>{});
+    const uint32_t v = (uint32_t)(16 / elem_size(m.a_elem));
+    const bool wide = m.k % v == 0 && m.a_stride % v == 0 && aligned_to(m.a, 16);
+    auto with_pieces = [&](auto T, auto V) { return wide ? with_gate(T, V) : with_gate(T, integral_constant<int, 1>{}); };
+    return m.a_elem == ELEM_F32 ? with_pieces(float{}, integral_constant<int, 4>{})
+           : m.a_elem == ELEM_BF16 ? with_pieces(__nv_bfloat16{}, integral_constant<int, 8>{}) : with_pieces(__half{}, integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -165,25 +188,22 @@ int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride
     }
     if (!on_current_device({a, a_scales, b, b_scales, expert_begin, out, coded ? nullptr : workspace})) return NVMAI_CUDA_EINVAL;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    MatmulParams p{};
-    p.rows = rows; p.k = k;
-    p.b = static_cast<const int8_t *>(b); p.b_stride = b_stride; p.b_scales = b_scales;
-    p.n = n; p.channels = (uint32_t)channels; p.E = num_experts; p.begin = expert_begin; p.act = activation;
-    p.out = out; p.out_elem = out_elem; p.out_stride = out_stride;
-    if (coded) {
-        p.a = static_cast<const int8_t *>(a); p.a_stride = a_stride; p.a_scales = a_scales;
-    } else {
+    Matmul m{a, a_elem, a_stride, a_scales, rows, k, static_cast<const int8_t *>(b), b_stride, b_scales, n, (uint32_t)channels,
+             num_experts, expert_begin, activation, out, out_elem, out_stride};
+    auto launched = [](cudaError_t e) {
+        count_launches(1);
+        if (e != cudaSuccess) cudaGetLastError();
+        return e == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
+    };
+    if (const uint32_t nt = stream_tiles(m)) return launched(launch_stream(m, nt, st));
+    if (!coded) {
         int8_t *q = static_cast<int8_t *>(workspace);
         float *scales = reinterpret_cast<float *>(q + scales_offset(rows, k));
-        const cudaError_t e = launch_quantize(a, a_elem, a_stride, rows, k, q, (uint32_t)code_stride(k), scales, st);
-        count_launches(1);
-        if (e != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
-        p.a = q; p.a_stride = code_stride(k); p.a_scales = scales;
+        const int rc = launched(launch_quantize(a, a_elem, a_stride, rows, k, q, (uint32_t)code_stride(k), scales, st));
+        if (rc) return rc;
+        m.a = q; m.a_stride = code_stride(k); m.a_scales = scales;
     }
-    const cudaError_t e = rows > 8 ? launch_gemm(p, st) : launch_pdl(int8_matmul_kernel, dim3(rows, (n + 7) / 8), dim3(256), 0, st, true, p);
-    count_launches(1);
-    if (e != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
-    return NVMAI_CUDA_OK;
+    return launched(launch_gemm(m, st));
 }
 
 int nvmai_cuda_moe_int8_matmul_status(void *stream) {

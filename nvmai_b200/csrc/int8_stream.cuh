@@ -1,0 +1,201 @@
+// Products of a few rows with matrices of 8-bit codes: the codes go from HBM to mma.sync once, nothing is staged.
+//
+// A block has 16 channels (with an activation: 8 gate rows and the 8 up rows of the same features, so that one thread has
+// both sums of an output) of one matrix and up to 8 NT rows.  Its eight warps split K; a lane fetches 16 neighbouring codes of
+// two channels at a time and uses them as two K steps of m16n8k32: the order of K inside a step is free as long as both
+// operands share it.  Rows that come as 16- or 32-bit elements are quantised by every block that needs them, which costs
+// less than a launch.  The sums are whole numbers, so neither the split nor the order changes a bit.
+#pragma once
+#include "common.cuh"
+#include "int8_gemm.cuh"
+#include "row_elem.cuh"
+#include "tma.cuh"
+
+namespace nvmai {
+
+constexpr int kIsThreads = 256, kIsWarps = 8;
+constexpr uint32_t kIsStep = 64;             // codes of a row that a warp uses at a time
+
+struct IsParams {
+    const void *a; size_t a_stride; const float *a_scales;
+    uint32_t rows, k;
+    const int8_t *b; size_t b_stride; const float *b_scales;
+    uint32_t n, channels, E;
+    const uint32_t *begin;
+    uint32_t act;
+    void *out; uint32_t out_elem; size_t out_stride;
+    uint32_t row_bytes;                      // a row of codes in shared memory
+};
+
+// Codes are zero from k to the end of the last step.  64 bytes more than a multiple of 128: two rows of a fragment
+// load cover all banks.
+__host__ __device__ constexpr uint32_t is_row_bytes(uint32_t k) {
+    const uint32_t steps = (k + kIsStep - 1) / kIsStep * kIsStep;
+    return steps % 128 == 0 ? steps + 64 : steps;
+}
+__host__ __device__ constexpr size_t is_smem(uint32_t k, uint32_t nt) { return (size_t)is_row_bytes(k) * 8 * nt + (size_t)kIsWarps * nt * 512; }
+
+__device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 codes of a channel from position i on; what is behind k reads as 0 and is not touched
+__device__ __forceinline__ uint4 codes16(const int8_t *row, uint32_t i, uint32_t k) {
+    if (i + 16u <= k) return ldg_stream_u4(row + i);
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (uint32_t j = 0; i + j < k; ++j) w[j / 4] |= (uint32_t)(uint8_t)row[i + j] << (8 * (j % 4));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// T: type of the rows (int8_t: codes with a_scales).  V: elements of a row read at once.
+template <typename T, int V, bool GATED, int NT>
+__global__ void __launch_bounds__(kIsThreads) int8_stream_kernel(IsParams p) {
+    constexpr bool kCoded = sizeof(T) == 1;
+    constexpr uint32_t kRows = 8 * NT;
+    extern __shared__ __align__(16) unsigned char is_smem_raw[];
+    __shared__ float scale[kRows], inverse[kRows];
+    __shared__ uint32_t top[kRows];
+    unsigned char *codes = is_smem_raw;
+    int *partial = reinterpret_cast<int *>(is_smem_raw + (size_t)p.row_bytes * kRows);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // the rows: every kRows-th one of an expert has a block column of its own
+    uint32_t row0 = blockIdx.y * kRows, e = 0, end = p.rows;
+    if (p.begin != nullptr) {
+        row0 = blockIdx.y;
+        uint32_t count = 0;
+        for (uint32_t i = tid; i <= p.E; i += kIsThreads) count += p.begin[i] <= row0 ? 1u : 0u;
+        if (tid < kRows) top[tid] = 0u;
+        __syncthreads();
+        count = __reduce_add_sync(0xffffffffu, count);
+        if (lane == 0) atomicAdd(&top[0], count);
+        __syncthreads();
+        e = top[0];                                            // begins up to this row
+        if (e == 0u || e > p.E) return;
+        --e;
+        end = min(p.begin[e + 1], p.rows);
+        const uint32_t first = p.begin[e];
+        if (first > row0 || row0 >= end || (row0 - first) % kRows != 0u) return;
+        __syncthreads();
+    }
+    const uint32_t count = min(end - row0, kRows);
+
+    // channels g and g + 8 of the block's sixteen
+    const uint32_t j0 = blockIdx.x * (GATED ? 8u : 16u), j = j0 + g;
+    const uint32_t c0 = j, c1 = GATED ? p.n + j : j + 8u;
+    const bool live0 = j < p.n, live1 = GATED ? live0 : j + 8u < p.n;
+    const int8_t *b0 = p.b + ((size_t)e * p.channels + (live0 ? c0 : 0u)) * p.b_stride;
+    const int8_t *b1 = p.b + ((size_t)e * p.channels + (live1 ? c1 : 0u)) * p.b_stride;
+    constexpr uint32_t kAhead = 4;                             // steps whose codes are requested together
+    const uint32_t steps = (p.k + kIsStep - 1u) / kIsStep;
+    uint4 w0[kAhead], w1[kAhead];
+    auto request = [&](uint32_t s0) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t s = s0 + i * kIsWarps, at = s * kIsStep + t * 16u;
+            w0[i] = s < steps && live0 ? codes16(b0, at, p.k) : make_uint4(0, 0, 0, 0);
+            w1[i] = s < steps && live1 ? codes16(b1, at, p.k) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    request(warp);
+
+    // the rows' codes to shared memory, zeros behind k and for rows that are not there
+    const T *a = static_cast<const T *>(p.a) + (size_t)row0 * p.a_stride;
+    const uint32_t pieces = p.k / V, padded = steps * kIsStep;
+    using P = Piece<T, V>;
+    using Q = Piece<int8_t, V>;
+    if constexpr (kCoded) {
+        for (uint32_t r = 0; r < kRows; ++r) {
+            const int8_t *src = reinterpret_cast<const int8_t *>(a) + (size_t)r * p.a_stride;
+            for (uint32_t i = tid * 16u; i < padded; i += kIsThreads * 16u)
+                *reinterpret_cast<uint4 *>(codes + r * p.row_bytes + i) = r < count && i < p.k ? codes16(src, i, p.k) : make_uint4(0, 0, 0, 0);
+        }
+        if (tid < kRows) scale[tid] = tid < count ? p.a_scales[row0 + tid] : 0.0f;
+    } else {
+        if (tid < kRows) top[tid] = 0u;
+        __syncthreads();
+        for (uint32_t r = 0; r < count; ++r) {
+            const P *src = reinterpret_cast<const P *>(a + (size_t)r * p.a_stride);
+            uint32_t m = 0;
+            for (uint32_t i = tid; i < pieces; i += kIsThreads) {
+                const P v = src[i];
+#pragma unroll
+                for (int x = 0; x < V; ++x) m = max(m, magnitude_bits(elem_to_float(v.v[x])));
+            }
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) atomicMax(&top[r], m);
+        }
+        __syncthreads();
+        if (tid < kRows) {
+            const RowScale rs = row_scale_bits(top[tid]);
+            scale[tid] = rs.scale;
+            inverse[tid] = rs.inverse;
+        }
+        __syncthreads();
+        for (uint32_t r = 0; r < kRows; ++r) {
+            const RowScale rs{0.0f, inverse[r]};
+            const P *src = reinterpret_cast<const P *>(a + (size_t)r * p.a_stride);
+            for (uint32_t i = tid; i < padded / V; i += kIsThreads) {
+                Q q;
+                if (r < count && i < pieces) {
+                    const P v = src[i];
+#pragma unroll
+                    for (int x = 0; x < V; ++x) q.v[x] = row_code(elem_to_float(v.v[x]), rs);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < V; ++x) q.v[x] = 0;
+                }
+                *reinterpret_cast<Q *>(codes + r * p.row_bytes + i * V) = q;
+            }
+        }
+    }
+    __syncthreads();
+
+    int acc[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) acc[x][0] = acc[x][1] = acc[x][2] = acc[x][3] = 0;
+    for (uint32_t s0 = warp; s0 < steps; s0 += kAhead * kIsWarps) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t s = s0 + i * kIsWarps;
+            if (s < steps) {
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    const uint4 y = *reinterpret_cast<const uint4 *>(codes + (8u * x + g) * p.row_bytes + s * kIsStep + t * 16u);
+                    mma_i8(acc[x], w0[i].x, w1[i].x, w0[i].y, w1[i].y, y.x, y.y);
+                    mma_i8(acc[x], w0[i].z, w1[i].z, w0[i].w, w1[i].w, y.z, y.w);
+                }
+            }
+        }
+        if (s0 + kAhead * kIsWarps < steps) request(s0 + kAhead * kIsWarps);
+    }
+    // the warps' parts of the sums: [warp][tile of 8 rows][lane][4]
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+        *reinterpret_cast<int4 *>(partial + ((warp * NT + x) * 32u + lane) * 4u) = make_int4(acc[x][0], acc[x][1], acc[x][2], acc[x][3]);
+    __syncthreads();
+    // out: consecutive threads take consecutive features of a row
+    constexpr uint32_t kOuts = GATED ? 8u : 16u;
+    const float *bs = p.b_scales + (size_t)e * p.channels;
+    for (uint32_t i = tid; i < kOuts * kRows; i += kIsThreads) {
+        const uint32_t f = i % kOuts, r = i / kOuts;
+        if (r >= count || j0 + f >= p.n) continue;
+        // row r is column r % 8 of tile r / 8: lane 4 (f % 8) + (r % 8) / 2, values r % 2 (channel f) and 2 + r % 2 (f + 8)
+        const uint32_t at = ((r / 8u) * 32u + 4u * (f % 8u) + (r % 8u) / 2u) * 4u + (r % 2u) + (!GATED && f >= 8u ? 2u : 0u);
+        int v = 0, u = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kIsWarps; ++w) {
+            v += partial[w * NT * 128u + at];
+            if (GATED) u += partial[w * NT * 128u + at + 2u];
+        }
+        float x = (scale[r] * bs[j0 + f]) * (float)v;
+        if (GATED) x = (p.out_elem == ELEM_F32 ? gate_act<false>(x, p.act) : gate_act<true>(x, p.act)) * ((scale[r] * bs[p.n + j0 + f]) * (float)u);
+        store_elem(p.out, p.out_elem, (size_t)(row0 + r) * p.out_stride + j0 + f, x);
+    }
+}
+
+}  // namespace nvmai

@@ -16,11 +16,17 @@ template <> __device__ __forceinline__ __half elem_from_float<__half>(float v) {
 template <> __device__ __forceinline__ float elem_from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 elem_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// element i of an array whose type is known at run time only (routing weights)
+// element i of an array whose type is known at run time only (routing weights, outputs of small calls)
 __device__ __forceinline__ float load_elem(const void *p, uint32_t elem, size_t i) {
     if (elem == ELEM_F16) return __half2float(static_cast<const __half *>(p)[i]);
     if (elem == ELEM_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
     return static_cast<const float *>(p)[i];
+}
+
+__device__ __forceinline__ void store_elem(void *p, uint32_t elem, size_t i, float v) {
+    if (elem == ELEM_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else if (elem == ELEM_BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<float *>(p)[i] = v;
 }
 
 // V neighbouring elements, moved in one access (V * sizeof(T) <= 16 bytes, aligned to that)
