@@ -21,7 +21,7 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // block has a run of tokens; it counts the experts of all pairs, those in front of its run apart, and ranks its own pairs
 // with one warp, 32 at a time (__match_any_sync gives the pairs of the same expert).  Then its warps move the tokens' rows.
 constexpr int kSortThreads = 1024;
-constexpr uint32_t kSortBlocks = 148;
+constexpr uint32_t kSms = 148, kSortBlocks = kSms;
 
 struct SortParams {
     const uint32_t *idx; uint32_t tokens, top_k, E;
@@ -155,45 +155,171 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
 
 // ---- merge_rows -----------------------------------------------------------------------------------------
 struct MergeParams {
-    const void *rows; size_t rows_stride; uint32_t n_rows;
+    const void *rows; uint32_t rows_stride, n_rows;
     const uint32_t *position; const void *w; uint32_t w_elem;
     uint32_t tokens, top_k, d;
     const void *base; size_t base_stride;
     void *y; size_t y_stride;
 };
 
-// A thread sums V neighbouring elements of one token over its slots.
-template <typename T, int V>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
+    if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A warp sums a run of 32 R pieces of V neighbouring elements of a token and goes on to the next run, as many warps further as
+// there are.  A step is a run's pieces of up to eight slots; a step is copied into shared memory while the one before is
+// added, each lane its own pieces, so that a lane waits for its own copies alone (cp.async groups) and no registers hold what is
+// in flight: 24 warps an SM with a step of 4 KB each.  4096 tokens of eight 4 KB rows on a B200: 26.6 us, 5.7 TB/s; a thread per piece
+// without the ring 35.2 (the rows' latency is exposed), a ring of four steps 56 (12 warps an SM, too few for the instructions).
+constexpr uint32_t kMergeSlots = 8, kMergeAhead = 2;
+__host__ __device__ constexpr uint32_t merge_stage_bytes(uint32_t top_k, uint32_t run_bytes) {
+    return (top_k < kMergeSlots ? top_k : kMergeSlots) * run_bytes;
+}
+
+template <typename T, int V, int R>
 __global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
     using P = Piece<T, V>;
+    constexpr int kPiece = sizeof(P);
+    constexpr uint32_t kRun = 32u * R, kRunBytes = kRun * kPiece;
+    extern __shared__ __align__(16) unsigned char merge_smem[];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t stage_bytes = merge_stage_bytes(p.top_k, kRunBytes);
+    unsigned char *ring = merge_smem + warp * kMergeAhead * stage_bytes + lane * kPiece;
+    const uint32_t ring_at = smem_addr(ring);
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t t = blockIdx.x * blockDim.y + threadIdx.y;
-    if (t >= p.tokens) return;
-    const uint32_t *pos = p.position + (size_t)t * p.top_k;
-    for (uint32_t c = threadIdx.x; c < p.d / V; c += blockDim.x) {
-        float acc[V];
-        if (p.base != nullptr) {
-            const P b = reinterpret_cast<const P *>(static_cast<const T *>(p.base) + (size_t)t * p.base_stride)[c];
+    const uint32_t pieces = p.d / V, runs = (pieces + kRun - 1u) / kRun, groups = (p.top_k + kMergeSlots - 1u) / kMergeSlots;
+    const uint32_t stride_t = gridDim.x * 8u / runs, stride_run = gridDim.x * 8u % runs;
+    const T *rows = static_cast<const T *>(p.rows);
+    struct At { uint32_t t, run, g; };
+    auto next = [&](At &x) {
+        if (++x.g < groups) return;
+        x.g = 0u;
+        x.t += stride_t;
+        if ((x.run += stride_run) >= runs) { x.run -= runs; ++x.t; }
+    };
+    // lane k: position of the step's slot k
+    auto position = [&](const At &x) {
+        const uint32_t k = x.g * kMergeSlots + lane;
+        return x.t < p.tokens && lane < kMergeSlots && k < p.top_k ? p.position[(size_t)x.t * p.top_k + k] : kNoRow;
+    };
+    auto request = [&](const At &x, uint32_t pos, uint32_t slot) {
+        const uint32_t c = x.run * kRun + lane, to = ring_at + slot * stage_bytes;
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = elem_to_float(b.v[i]);
-        } else {
+        for (uint32_t k = 0; k < kMergeSlots; ++k) {
+            const uint32_t row = __shfl_sync(0xffffffffu, pos, k);
+            if (row < p.n_rows) {
+                const P *src = reinterpret_cast<const P *>(rows + (size_t)row * p.rows_stride) + c;
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+                for (uint32_t r = 0; r < R; ++r)
+                    if (c + r * 32u < pieces) cp_async(to + k * kRunBytes + r * 32u * kPiece, src + r * 32u, kPiece);
+            }
         }
-#pragma unroll 8
-        for (uint32_t k = 0; k < p.top_k; ++k) {
-            const uint32_t row = pos[k];
-            if (row >= p.n_rows) continue;
-            const float w = p.w != nullptr ? load_elem(p.w, p.w_elem, (size_t)t * p.top_k + k) : 1.0f;
-            const P v = reinterpret_cast<const P *>(static_cast<const T *>(p.rows) + (size_t)row * p.rows_stride)[c];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const uint32_t first = blockIdx.x * 8u + warp;
+    At now{first / runs, first % runs, 0u}, head = now;      // the step to add and the one to request
+    next(head);
+    uint32_t now_pos = position(now), head_pos = position(head);
+    request(now, now_pos, 0u);
+    float acc[R][V];
+    for (uint32_t slot = 0; now.t < p.tokens; slot ^= 1u) {
+        At then = head;
+        next(then);
+        const uint32_t then_pos = position(then);
+        request(head, head_pos, slot ^ 1u);                  // into the slot that the last round emptied
+        const uint32_t c = now.run * kRun + lane;
+        if (now.g == 0u) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, elem_to_float(v.v[i]), acc[i]);
+            for (uint32_t r = 0; r < R; ++r) {
+                P b;
+                const bool has = p.base != nullptr && c + r * 32u < pieces;
+                if (has) b = reinterpret_cast<const P *>(static_cast<const T *>(p.base) + (size_t)now.t * p.base_stride)[c + r * 32u];
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[r][i] = has ? elem_to_float(b.v[i]) : 0.0f;
+            }
         }
-        P o;
+        const bool weighs = p.w != nullptr && lane < kMergeSlots && now_pos < p.n_rows;
+        const float mine = weighs ? load_elem(p.w, p.w_elem, (size_t)now.t * p.top_k + now.g * kMergeSlots + lane) : 1.0f;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMergeAhead - 1) : "memory");
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = elem_from_float<T>(acc[i]);
-        reinterpret_cast<P *>(static_cast<T *>(p.y) + (size_t)t * p.y_stride)[c] = o;
+        for (uint32_t k = 0; k < kMergeSlots; ++k) {
+            const uint32_t row = __shfl_sync(0xffffffffu, now_pos, k);
+            const float w = __shfl_sync(0xffffffffu, mine, k);
+            if (row < p.n_rows) {
+#pragma unroll
+                for (uint32_t r = 0; r < R; ++r) {
+                    if (c + r * 32u >= pieces) continue;
+                    const P v = *reinterpret_cast<const P *>(ring + slot * stage_bytes + k * kRunBytes + r * 32u * kPiece);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[r][i] = fmaf(w, elem_to_float(v.v[i]), acc[r][i]);
+                }
+            }
+        }
+        if (now.g + 1u == groups) {
+#pragma unroll
+            for (uint32_t r = 0; r < R; ++r) {
+                if (c + r * 32u >= pieces) continue;
+                P o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.v[i] = elem_from_float<T>(acc[r][i]);
+                reinterpret_cast<P *>(static_cast<T *>(p.y) + (size_t)now.t * p.y_stride)[c + r * 32u] = o;
+            }
+        }
+        now = head;
+        now_pos = head_pos;
+        head = then;
+        head_pos = then_pos;
+    }
+}
+
+// Rows of 16-bit elements that share no 4-byte boundary: a thread sums every 32nd element, four of them and two slots at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) merge_narrow_kernel(MergeParams p) {
+    constexpr int U = 4, kAhead = 2;
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t t = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31u;
+    if (t >= p.tokens) return;                             // whole warps: a block row is a multiple of 32 threads
+    const T *rows = static_cast<const T *>(p.rows);
+    for (uint32_t c0 = threadIdx.x; c0 - lane < p.d; c0 += blockDim.x * U) {
+        float acc[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t c = c0 + u * blockDim.x;
+            acc[u] = p.base != nullptr && c < p.d ? elem_to_float(static_cast<const T *>(p.base)[(size_t)t * p.base_stride + c]) : 0.0f;
+        }
+        for (uint32_t k0 = 0; k0 < p.top_k; k0 += 32u) {
+            const size_t pair = (size_t)t * p.top_k + k0 + lane;
+            const uint32_t mine = k0 + lane < p.top_k ? p.position[pair] : kNoRow;
+            const float mine_w = mine < p.n_rows && p.w != nullptr ? load_elem(p.w, p.w_elem, pair) : 1.0f;
+            for (uint32_t s = 0; s < min(p.top_k - k0, 32u); s += kAhead) {
+                T v[kAhead][U];
+                uint32_t row[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    row[j] = s + j < 32u ? __shfl_sync(0xffffffffu, mine, s + j) : kNoRow;      // lanes past the slots hold kNoRow
+                    if (row[j] < p.n_rows) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (c0 + u * blockDim.x < p.d) v[j][u] = rows[(size_t)row[j] * p.rows_stride + c0 + u * blockDim.x];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const float w = __shfl_sync(0xffffffffu, mine_w, (s + j) & 31u);
+                    if (row[j] < p.n_rows) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (c0 + u * blockDim.x < p.d) acc[u] = fmaf(w, elem_to_float(v[j][u]), acc[u]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * blockDim.x < p.d) static_cast<T *>(p.y)[(size_t)t * p.y_stride + c0 + u * blockDim.x] = elem_from_float<T>(acc[u]);
     }
 }
 
@@ -224,7 +350,8 @@ __global__ void __launch_bounds__(256) merge_rows_grad_kernel(MergeGradParams p)
     const P *v = reinterpret_cast<const P *>(static_cast<const T *>(p.rows) + (size_t)row * p.rows_stride);
     P *o = reinterpret_cast<P *>(static_cast<T *>(p.drows) + (size_t)row * p.drows_stride);
     float dot = 0.0f;
-#pragma unroll 4
+    constexpr int kUnroll = sizeof(P) == 16 ? 4 : 8;
+#pragma unroll kUnroll
     for (uint32_t c = lane; c < p.d / V; c += 32u) {
         const P g = dy[c];
         if (p.dw != nullptr) {
@@ -265,14 +392,15 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p) {
     const P *src = reinterpret_cast<const P *>(static_cast<const T *>(p.x) + (size_t)row * p.x_stride);
     Q *dst = reinterpret_cast<Q *>(p.q + (size_t)row * p.q_stride);
     uint32_t m = 0;
-#pragma unroll 4
+    constexpr int kUnroll = sizeof(P) == 16 ? 4 : 8;
+#pragma unroll kUnroll
     for (uint32_t c = lane; c < p.n / V; c += 32u) {
         const P v = src[c];
 #pragma unroll
         for (int i = 0; i < V; ++i) m = max(m, magnitude_bits(elem_to_float(v.v[i])));
     }
     const RowScale rs = row_scale_bits(__reduce_max_sync(0xffffffffu, m));
-#pragma unroll 4
+#pragma unroll kUnroll
     for (uint32_t c = lane; c < p.n / V; c += 32u) {
         const P v = src[c];
         Q q;
@@ -291,19 +419,24 @@ int launched(cudaError_t e) {
     return e == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
 }
 
-// Elements a thread moves at once: 16 bytes where every buffer starts on such a boundary, its rows are that far apart
-// and a row is a whole number of them; one element otherwise.
+// Elements a thread moves at once: as many as make 16 bytes where every buffer starts on such a boundary, its rows are that far
+// apart and a row is a whole number of them; two of 16 bits by the same rule; else one.
 struct Rows { const void *p; size_t stride, size; };
+bool on_boundary(std::initializer_list<Rows> rows, size_t v) {
+    for (const Rows &r : rows)
+        if (r.p != nullptr && (r.stride % v != 0 || !aligned_to(r.p, v * r.size))) return false;
+    return true;
+}
 template <typename F>
 auto with_pieces(uint32_t elem, uint32_t d, std::initializer_list<Rows> rows, F &&f) {
-    const size_t v = 16 / elem_size(elem);
-    bool wide = d % v == 0;
-    for (const Rows &r : rows)
-        if (r.p != nullptr) wide = wide && r.stride % v == 0 && aligned_to(r.p, std::min<size_t>(16, v * r.size));
+    const size_t most = 16 / elem_size(elem);
+    const size_t v = d % most == 0 && on_boundary(rows, most) ? most : d % 2 == 0 && on_boundary(rows, 2) ? 2 : 1;
     using std::integral_constant;
-    if (elem == ELEM_F32) return wide ? f(float{}, integral_constant<int, 4>{}) : f(float{}, integral_constant<int, 1>{});
-    if (elem == ELEM_BF16) return wide ? f(__nv_bfloat16{}, integral_constant<int, 8>{}) : f(__nv_bfloat16{}, integral_constant<int, 1>{});
-    return wide ? f(__half{}, integral_constant<int, 8>{}) : f(__half{}, integral_constant<int, 1>{});
+    auto with_16 = [&](auto T) {
+        return v == 8 ? f(T, integral_constant<int, 8>{}) : v == 2 ? f(T, integral_constant<int, 2>{}) : f(T, integral_constant<int, 1>{});
+    };
+    if (elem == ELEM_F32) return v == 4 ? f(float{}, integral_constant<int, 4>{}) : f(float{}, integral_constant<int, 1>{});
+    return elem == ELEM_BF16 ? with_16(__nv_bfloat16{}) : with_16(__half{});
 }
 
 }  // namespace
@@ -362,14 +495,29 @@ int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_t rows_str
     if (tokens == 0) return NVMAI_CUDA_OK;
     if (!on_current_device({n_rows != 0 ? rows : nullptr, position, w, base, y})) return NVMAI_CUDA_EINVAL;
     const MergeParams p{rows, rows_stride, n_rows, position, w, w_elem, tokens, top_k, d, base, base_stride, y, y_stride};
-    return with_pieces(elem, d, {{n_rows != 0 ? rows : nullptr, rows_stride, size}, {base, base_stride, size}, {y, y_stride, size}}, [&](auto T, auto V) {
-        constexpr int v = decltype(V)::value;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const std::initializer_list<Rows> all{{n_rows != 0 ? rows : nullptr, rows_stride, size}, {base, base_stride, size}, {y, y_stride, size}};
+    auto narrow = [&](auto T) {
         uint32_t tx = 32;
-        while (tx < 256 && tx < d / v) tx *= 2;
+        while (tx < 256 && tx * 4 < d) tx *= 2;
         const uint32_t ty = 256 / tx;
-        return launched(launch_pdl(merge_rows_kernel<decltype(T), v>, dim3((tokens + ty - 1) / ty), dim3(tx, ty), 0,
-                                   static_cast<cudaStream_t>(stream), true, p));
-    });
+        return launched(launch_pdl(merge_narrow_kernel<decltype(T)>, dim3((tokens + ty - 1) / ty), dim3(tx, ty), 0, st, true, p));
+    };
+    auto go = [&](auto T, auto V) {
+        using std::integral_constant;
+        constexpr uint32_t piece = sizeof(T) * decltype(V)::value;
+        if constexpr (piece < 4) {
+            return narrow(T);
+        } else {
+            constexpr int r = piece == 16 ? 1 : 4;               // 4-byte pieces: four times as many of them a step
+            const size_t smem = 8 * kMergeAhead * (size_t)merge_stage_bytes(top_k, 32 * r * piece);
+            const uint64_t runs = (uint64_t)tokens * ((d / decltype(V)::value + 32 * r - 1) / (32 * r));
+            const uint64_t resident = kSms * std::min<uint64_t>(8, 220 * 1024 / (smem + 1024));
+            return launched(launch_pdl(merge_rows_kernel<decltype(T), decltype(V)::value, r>, dim3((unsigned)std::min<uint64_t>(resident, (runs + 7) / 8)),
+                                       dim3(256), smem, st, true, p));
+        }
+    };
+    return with_pieces(elem, d, all, go);
 }
 
 int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_stride, const void *rows, uint32_t rows_stride,
