@@ -26,6 +26,7 @@ struct IgParams {
     void *out; size_t out_stride;
     uint32_t nt, stages;                 // most rows of a unit (a multiple of 32), ring slots
     uint32_t accs;                       // sets of accumulators (2, or 1 where two do not fit)
+    uint32_t ready;                      // the kernel in front made the rows' codes and nothing else that is read here
     uint32_t paired;                     // 16-bit outputs: two neighbouring channels go out in one store
     uint32_t channel_tiles;              // units across the channels
     unsigned int *status;
@@ -130,8 +131,11 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
         tmem_relinquish();
     }
     if (warp == kIgCopyWarp && lane == 0) { tma_prefetch_map(&args.a); tma_prefetch_map(&args.b); }
-    pdl_wait();
-    pdl_launch_dependents();
+    auto wait_in_front = [&]() {
+        pdl_wait();
+        pdl_launch_dependents();
+    };
+    if (!p.ready) wait_in_front();
     // Row tiles in front of each expert: a thread adds up to four experts, the warps' sums are put together.  Begins behind
     // the last row or out of order give an expert fewer rows or none, never rows outside.
     {
@@ -192,18 +196,31 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
         if (elect_one()) {
             uint32_t stage = 0, parity = 1, filled = 0;         // the first pass finds every slot empty
             bool ok = true;
+            // channel tiles of a unit's K block; a unit's bytes are announced with them
+            auto load_channels = [&](const IgUnit &un, uint32_t kb, uint32_t at) {
+                const uint32_t boxes = (un.count + kIgBoxRows - 1u) / kIgBoxRows, slot = ring + at * stage_bytes;
+                const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : SUBS * 128u);
+                mbar_expect_tx(&s.full[at], SUBS * kIgTileBytes + boxes * kIgBoxRows * 128u);
+                tma_load_2d(slot, &args.b, kb * 128u, ch0, &s.full[at]);
+                if (SUBS == 2) tma_load_2d(slot + kIgTileBytes, &args.b, kb * 128u, GATED ? ch0 + p.n : ch0 + 128u, &s.full[at]);
+            };
+            uint32_t early = 0;                                  // K blocks whose channels are on their way before the rows can be
+            if (p.ready && blockIdx.x < total) {
+                const IgUnit un = ig_unit(s, p, blockIdx.x);
+                for (early = 0; early < min(n_kb, p.stages); ++early) load_channels(un, early, early);
+            }
+            if (p.ready) wait_in_front();
             for (uint32_t u = blockIdx.x; ok && u < total; u += gridDim.x) {
                 const IgUnit un = ig_unit(s, p, u);
                 const uint32_t boxes = (un.count + kIgBoxRows - 1u) / kIgBoxRows;
-                const uint32_t bytes = SUBS * kIgTileBytes + boxes * kIgBoxRows * 128u;
-                const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : SUBS * 128u);
-                const uint32_t ch1 = GATED ? ch0 + p.n : ch0 + 128u;
                 for (uint32_t kb = 0; kb < n_kb; ++kb) {
-                    if (!(ok = wait(&s.empty[stage], parity))) break;
                     const uint32_t slot = ring + stage * stage_bytes;
-                    mbar_expect_tx(&s.full[stage], bytes);
-                    tma_load_2d(slot, &args.b, kb * 128u, ch0, &s.full[stage]);
-                    if (SUBS == 2) tma_load_2d(slot + kIgTileBytes, &args.b, kb * 128u, ch1, &s.full[stage]);
+                    if (early != 0u) {
+                        --early;
+                    } else {
+                        if (!(ok = wait(&s.empty[stage], parity))) break;
+                        load_channels(un, kb, stage);
+                    }
                     for (uint32_t i = 0; i < boxes; ++i)
                         tma_load_2d(slot + SUBS * kIgTileBytes + i * kIgBoxRows * 128u, &args.a, kb * 128u, un.row + i * kIgBoxRows, &s.full[stage]);
                     ++filled;
@@ -258,6 +275,7 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
         const bool paired = kHalf && p.paired != 0u;
         float4 *scales = s.row_scales[warp];
         uint32_t it = 0;
+        if (p.ready) wait_in_front();
         for (uint32_t u = blockIdx.x; u < total; u += gridDim.x, ++it) {
             const IgUnit un = ig_unit(s, p, u);
             const uint32_t buf = p.accs == 2u ? it & 1u : 0u, turn = p.accs == 2u ? it >> 1 : it;

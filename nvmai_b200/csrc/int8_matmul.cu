@@ -29,6 +29,7 @@ struct Matmul {
     const uint32_t *begin;          // or nullptr: one matrix
     uint32_t act;
     void *out; uint32_t out_elem; size_t out_stride;
+    bool ready;                     // the call's own quantisation is the kernel in front
 };
 
 // codes and scales of rows that come as 16- or 32-bit elements
@@ -112,6 +113,7 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     p.channel_tiles = (m.n + (gated ? 128 : subs * 128) - 1) / (gated ? 128 : subs * 128);
     const size_t stage = subs * kIgTileBytes + (size_t)p.nt * 128;
     p.accs = 2 * subs * p.nt <= 512 ? 2 : 1;
+    p.ready = m.ready;
     p.paired = m.n % 2 == 0 && m.out_stride % 2 == 0 && aligned_to(m.out, 4);
     p.stages = (uint32_t)std::min<size_t>(kIgMaxStages, (227 * 1024 - sizeof(IgShared) - 2048) / stage);
     const size_t smem = 1024 + p.stages * stage;
@@ -126,19 +128,28 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     return m.out_elem == ELEM_F16 ? go(__half{}) : m.out_elem == ELEM_BF16 ? go(__nv_bfloat16{}) : go(float{});
 }
 
-// Rows that the streaming kernel takes: its blocks go through the codes once for every 8 to 32 rows.
+// The streaming kernel's tiles of 8 rows, 0: the tcgen05 kernel's.  One matrix: up to 32 rows (codes, 2048 -> 2 x 512 on a B200: 1 row
+// 3.2 us against 7.3, 16 rows 4.2 / 7.3, 32 rows 5.9 / 7.4).  By expert a block has the rows of one, and every one fetches
+// its codes anew: while rows x k is below 2^15 (8 rows of 2048: 6.4 / 10.0 us, 16 rows 11.3 / 11.6, 24 rows 15.7 / 14.0; 32 rows of 512
+// 10.1 / 10.5, 64 rows 16.4 / 14.9).
 uint32_t stream_tiles(const Matmul &m) {
+    if (m.begin != nullptr ? (uint64_t)m.rows * m.k >= 32768 || m.rows > 64 : m.rows > 32) return 0;
     const uint32_t nt = m.begin != nullptr || m.rows <= 8 ? 1 : m.rows <= 16 ? 2 : 4;
-    if (m.rows > (m.begin != nullptr ? 64u : 32u)) return 0;
     return is_smem(m.k, nt) <= 200 * 1024 ? nt : 0;
 }
+// Does it quantise the rows itself?  Each of its blocks then does, 0.6 us a row in front of the product; a launch for all of
+// them runs beside the fetching of the codes (2048 -> 2 x 512: 1 row 3.9 us in one launch, 4 rows 5.6, in two launches 4.6).
+bool stream_quantizes(const Matmul &m) { return m.begin != nullptr || m.rows <= 2; }
 
 cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
     using std::integral_constant;
     const bool gated = m.act != kActNone;
-    const IsParams p{m.a, m.a_stride, m.a_scales, m.rows, m.k, m.b, m.b_stride, m.b_scales, m.n, m.channels, m.E, m.begin, m.act,
-                     m.out, m.out_elem, m.out_stride, is_row_bytes(m.k)};
-    const dim3 grid((m.n + (gated ? 7 : 15)) / (gated ? 8 : 16), m.begin != nullptr ? m.rows : (m.rows + 8 * nt - 1) / (8 * nt));
+    IsParams p{m.a, m.a_stride, m.a_scales, m.rows, m.k, m.b, m.b_stride, m.b_scales, m.n, m.channels, m.E, m.begin, m.act,
+               m.out, m.out_elem, m.out_stride, m.ready, is_row_bytes(m.k), 1};
+    const uint32_t steps = (m.k + kIsStep - 1) / kIsStep, columns = m.begin != nullptr ? m.rows : (m.rows + 8 * nt - 1) / (8 * nt);
+    auto blocks = [&] { return (m.n * p.parts + (gated ? 8 : 16) * kIsWarps - 1) / ((gated ? 8 : 16) * kIsWarps); };    // across the features
+    while (p.parts < kIsWarps && p.parts < steps && (steps > p.parts * kIsAhead || (uint64_t)blocks() * columns < kSms)) p.parts *= 2;
+    const dim3 grid(blocks(), columns);
     auto go = [&](auto T, auto V, auto G, auto N) {
         return launch_pdl(int8_stream_kernel<decltype(T), decltype(V)::value, decltype(G)::value, decltype(N)::value>, grid,
                           dim3(kIsThreads), is_smem(m.k, nt), st, true, p);
@@ -151,11 +162,10 @@ cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
         return gated ? with_tiles(T, V, integral_constant<bool, true>{}) : with_tiles(T, V, integral_constant<bool, false>{});
     };
     if (m.a_elem == ELEM_I8) return with_gate(int8_t{}, integral_constant<int, 16>{});
-    const uint32_t v = (uint32_t)(16 / elem_size(m.a_elem));
-    const bool wide = m.k % v == 0 && m.a_stride % v == 0 && aligned_to(m.a, 16);
+    const bool wide = m.k % 4 == 0 && m.a_stride % 4 == 0 && aligned_to(m.a, 4 * elem_size(m.a_elem));     // four elements at once
     auto with_pieces = [&](auto T, auto V) { return wide ? with_gate(T, V) : with_gate(T, integral_constant<int, 1>{}); };
     return m.a_elem == ELEM_F32 ? with_pieces(float{}, integral_constant<int, 4>{})
-           : m.a_elem == ELEM_BF16 ? with_pieces(__nv_bfloat16{}, integral_constant<int, 8>{}) : with_pieces(__half{}, integral_constant<int, 8>{});
+           : m.a_elem == ELEM_BF16 ? with_pieces(__nv_bfloat16{}, integral_constant<int, 4>{}) : with_pieces(__half{}, integral_constant<int, 4>{});
 }
 
 }  // namespace
@@ -189,21 +199,21 @@ int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride
     if (!on_current_device({a, a_scales, b, b_scales, expert_begin, out, coded ? nullptr : workspace})) return NVMAI_CUDA_EINVAL;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Matmul m{a, a_elem, a_stride, a_scales, rows, k, static_cast<const int8_t *>(b), b_stride, b_scales, n, (uint32_t)channels,
-             num_experts, expert_begin, activation, out, out_elem, out_stride};
+             num_experts, expert_begin, activation, out, out_elem, out_stride, false};
     auto launched = [](cudaError_t e) {
         count_launches(1);
         if (e != cudaSuccess) cudaGetLastError();
         return e == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
     };
-    if (const uint32_t nt = stream_tiles(m)) return launched(launch_stream(m, nt, st));
-    if (!coded) {
+    const uint32_t nt = stream_tiles(m);
+    if (!coded && !(nt && stream_quantizes(m))) {
         int8_t *q = static_cast<int8_t *>(workspace);
         float *scales = reinterpret_cast<float *>(q + scales_offset(rows, k));
         const int rc = launched(launch_quantize(a, a_elem, a_stride, rows, k, q, (uint32_t)code_stride(k), scales, st));
         if (rc) return rc;
-        m.a = q; m.a_stride = code_stride(k); m.a_scales = scales;
+        m.a = q; m.a_elem = ELEM_I8; m.a_stride = code_stride(k); m.a_scales = scales; m.ready = true;
     }
-    return launched(launch_gemm(m, st));
+    return launched(nt ? launch_stream(m, nt, st) : launch_gemm(m, st));
 }
 
 int nvmai_cuda_moe_int8_matmul_status(void *stream) {

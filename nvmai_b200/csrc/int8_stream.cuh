@@ -1,7 +1,8 @@
 // Products of a few rows with matrices of 8-bit codes: the codes go from HBM to mma.sync once, nothing is staged.
 //
-// A block has 16 channels (with an activation: 8 gate rows and the 8 up rows of the same features, so that one thread has
-// both sums of an output) of one matrix and up to 8 NT rows.  Its eight warps split K; a lane fetches 16 neighbouring codes of
+// A warp has 16 channels (with an activation: 8 gate rows and the 8 up rows of the same features, so that one thread has
+// both sums of an output) of one matrix, up to 8 NT rows and a part of K: the block's sixteen warps split K until a part is short
+// (kIsAhead steps, all requested at once, or less where that gives every SM a block) and have different channels beyond that.  A lane fetches 16 neighbouring codes of
 // two channels at a time and uses them as two K steps of m16n8k32: the order of K inside a step is free as long as both
 // operands share it.  Rows that come as 16- or 32-bit elements are quantised by every block that needs them, which costs
 // less than a launch.  The sums are whole numbers, so neither the split nor the order changes a bit.
@@ -13,8 +14,9 @@
 
 namespace nvmai {
 
-constexpr int kIsThreads = 256, kIsWarps = 8;
+constexpr int kIsThreads = 512, kIsWarps = 16;
 constexpr uint32_t kIsStep = 64;             // codes of a row that a warp uses at a time
+constexpr uint32_t kIsAhead = 4;             // steps whose codes are requested together
 
 struct IsParams {
     const void *a; size_t a_stride; const float *a_scales;
@@ -24,7 +26,9 @@ struct IsParams {
     const uint32_t *begin;
     uint32_t act;
     void *out; uint32_t out_elem; size_t out_stride;
+    uint32_t ready;                          // the kernel in front made the rows' codes and nothing else that is read here
     uint32_t row_bytes;                      // a row of codes in shared memory
+    uint32_t parts;                          // of K: a power of two up to 16 warps
 };
 
 // Codes are zero from k to the end of the last step.  64 bytes more than a multiple of 128: two rows of a fragment
@@ -51,98 +55,119 @@ __device__ __forceinline__ uint4 codes16(const int8_t *row, uint32_t i, uint32_t
 
 // T: type of the rows (int8_t: codes with a_scales).  V: elements of a row read at once.
 template <typename T, int V, bool GATED, int NT>
-__global__ void __launch_bounds__(kIsThreads) int8_stream_kernel(IsParams p) {
+__global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kernel(IsParams p) {
     constexpr bool kCoded = sizeof(T) == 1;
-    constexpr uint32_t kRows = 8 * NT;
+    constexpr uint32_t kRows = 8 * NT, kFeatures = GATED ? 8 : 16;
     extern __shared__ __align__(16) unsigned char is_smem_raw[];
-    __shared__ float scale[kRows], inverse[kRows];
-    __shared__ uint32_t top[kRows];
+    __shared__ float scale[kRows];
+    __shared__ uint32_t top[kRows], found[3];
     unsigned char *codes = is_smem_raw;
     int *partial = reinterpret_cast<int *>(is_smem_raw + (size_t)p.row_bytes * kRows);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
-    pdl_wait();
-    pdl_launch_dependents();
+    using P = Piece<T, V>;
+    using Q = Piece<int8_t, V>;
+    if (tid < kRows) top[tid] = 0u;
+    if (tid == 0) found[0] = p.E;
+    __syncthreads();
+    auto wait_in_front = [&]() {
+        pdl_wait();
+        pdl_launch_dependents();
+    };
+    const bool ready = kCoded && p.ready != 0u;
+    if (!ready) wait_in_front();
 
     // the rows: every kRows-th one of an expert has a block column of its own
     uint32_t row0 = blockIdx.y * kRows, e = 0, end = p.rows;
+    const uint32_t pieces = p.k / V;
+    if (p.begin != nullptr) row0 = blockIdx.y;
+    const T *a = static_cast<const T *>(p.a) + (size_t)row0 * p.a_stride;
+    P early;                                                   // of the first row, on its way while the expert is looked up
+    if (!kCoded && tid < pieces) early = reinterpret_cast<const P *>(a)[tid];
     if (p.begin != nullptr) {
-        row0 = blockIdx.y;
-        uint32_t count = 0;
-        for (uint32_t i = tid; i <= p.E; i += kIsThreads) count += p.begin[i] <= row0 ? 1u : 0u;
-        if (tid < kRows) top[tid] = 0u;
+        for (uint32_t i = tid; i < p.E; i += kIsThreads) {
+            const uint32_t from = p.begin[i], to = p.begin[i + 1];
+            if (from <= row0 && row0 < to) { found[0] = i; found[1] = from; found[2] = to; }
+        }
         __syncthreads();
-        count = __reduce_add_sync(0xffffffffu, count);
-        if (lane == 0) atomicAdd(&top[0], count);
-        __syncthreads();
-        e = top[0];                                            // begins up to this row
-        if (e == 0u || e > p.E) return;
-        --e;
-        end = min(p.begin[e + 1], p.rows);
-        const uint32_t first = p.begin[e];
-        if (first > row0 || row0 >= end || (row0 - first) % kRows != 0u) return;
-        __syncthreads();
+        e = found[0];
+        if (e >= p.E || (row0 - found[1]) % kRows != 0u) {
+            if (ready) wait_in_front();
+            return;
+        }
+        end = min(found[2], p.rows);
     }
     const uint32_t count = min(end - row0, kRows);
 
-    // channels g and g + 8 of the block's sixteen
-    const uint32_t j0 = blockIdx.x * (GATED ? 8u : 16u), j = j0 + g;
+    // channels g and g + 8 of the warp's sixteen, and its part of K: every parts-th step
+    const uint32_t parts = p.parts, part = warp % parts, group = warp / parts, groups = kIsWarps / parts;
+    const uint32_t j0 = (blockIdx.x * groups + group) * kFeatures, j = j0 + g;
     const uint32_t c0 = j, c1 = GATED ? p.n + j : j + 8u;
     const bool live0 = j < p.n, live1 = GATED ? live0 : j + 8u < p.n;
     const int8_t *b0 = p.b + ((size_t)e * p.channels + (live0 ? c0 : 0u)) * p.b_stride;
     const int8_t *b1 = p.b + ((size_t)e * p.channels + (live1 ? c1 : 0u)) * p.b_stride;
-    constexpr uint32_t kAhead = 4;                             // steps whose codes are requested together
     const uint32_t steps = (p.k + kIsStep - 1u) / kIsStep;
-    uint4 w0[kAhead], w1[kAhead];
+    const bool whole = p.k % 16u == 0u;                        // no piece of 16 codes ends inside
+    uint4 w0[kIsAhead], w1[kIsAhead];
     auto request = [&](uint32_t s0) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t s = s0 + i * kIsWarps, at = s * kIsStep + t * 16u;
-            w0[i] = s < steps && live0 ? codes16(b0, at, p.k) : make_uint4(0, 0, 0, 0);
-            w1[i] = s < steps && live1 ? codes16(b1, at, p.k) : make_uint4(0, 0, 0, 0);
+        for (uint32_t i = 0; i < kIsAhead; ++i) {
+            const uint32_t s = s0 + i * parts, at = s * kIsStep + t * 16u;
+            w0[i] = w1[i] = make_uint4(0, 0, 0, 0);
+            if (whole) {
+                if (at < p.k && live0) w0[i] = ldg_stream_u4(b0 + at);
+                if (at < p.k && live1) w1[i] = ldg_stream_u4(b1 + at);
+            } else if (s < steps) {
+                if (live0) w0[i] = codes16(b0, at, p.k);
+                if (live1) w1[i] = codes16(b1, at, p.k);
+            }
         }
     };
-    request(warp);
+    request(part);
+    if (ready) wait_in_front();
 
-    // the rows' codes to shared memory, zeros behind k and for rows that are not there
-    const T *a = static_cast<const T *>(p.a) + (size_t)row0 * p.a_stride;
-    const uint32_t pieces = p.k / V, padded = steps * kIsStep;
-    using P = Piece<T, V>;
-    using Q = Piece<int8_t, V>;
+    // the rows' codes to shared memory, zeros behind k; rows that are not there stay what they are (their columns are not stored)
+    const uint32_t padded = steps * kIsStep;
     if constexpr (kCoded) {
-        for (uint32_t r = 0; r < kRows; ++r) {
-            const int8_t *src = reinterpret_cast<const int8_t *>(a) + (size_t)r * p.a_stride;
-            for (uint32_t i = tid * 16u; i < padded; i += kIsThreads * 16u)
-                *reinterpret_cast<uint4 *>(codes + r * p.row_bytes + i) = r < count && i < p.k ? codes16(src, i, p.k) : make_uint4(0, 0, 0, 0);
+        const uint32_t each = padded / 16u;
+        for (uint32_t i = tid; i < each * count; i += kIsThreads) {
+            const uint32_t r = i / each, c = (i - r * each) * 16u;
+            *reinterpret_cast<uint4 *>(codes + r * p.row_bytes + c) =
+                c < p.k ? codes16(reinterpret_cast<const int8_t *>(a) + (size_t)r * p.a_stride, c, p.k) : make_uint4(0, 0, 0, 0);
         }
-        if (tid < kRows) scale[tid] = tid < count ? p.a_scales[row0 + tid] : 0.0f;
+        if (tid < count) scale[tid] = p.a_scales[row0 + tid];
     } else {
-        if (tid < kRows) top[tid] = 0u;
+        auto largest = [&](const P &v, uint32_t m) {
+#pragma unroll
+            for (int x = 0; x < V; ++x) m = max(m, magnitude_bits(elem_to_float(v.v[x])));
+            return m;
+        };
+        for (uint32_t r0 = 0; r0 < count; r0 += 4u) {          // four rows' pieces on their way at a time
+            uint32_t m[4] = {0, 0, 0, 0};
+            for (uint32_t i = tid; i < pieces; i += kIsThreads) {
+                P v[4];
+#pragma unroll
+                for (uint32_t x = 0; x < 4u; ++x)
+                    if (r0 + x < count) v[x] = r0 + x == 0u && i == tid ? early : reinterpret_cast<const P *>(a + (size_t)(r0 + x) * p.a_stride)[i];
+#pragma unroll
+                for (uint32_t x = 0; x < 4u; ++x)
+                    if (r0 + x < count) m[x] = largest(v[x], m[x]);
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < 4u; ++x)
+                if (r0 + x < count) {
+                    m[x] = __reduce_max_sync(0xffffffffu, m[x]);
+                    if (lane == 0) atomicMax(&top[r0 + x], m[x]);
+                }
+        }
         __syncthreads();
         for (uint32_t r = 0; r < count; ++r) {
-            const P *src = reinterpret_cast<const P *>(a + (size_t)r * p.a_stride);
-            uint32_t m = 0;
-            for (uint32_t i = tid; i < pieces; i += kIsThreads) {
-                const P v = src[i];
-#pragma unroll
-                for (int x = 0; x < V; ++x) m = max(m, magnitude_bits(elem_to_float(v.v[x])));
-            }
-            m = __reduce_max_sync(0xffffffffu, m);
-            if (lane == 0) atomicMax(&top[r], m);
-        }
-        __syncthreads();
-        if (tid < kRows) {
-            const RowScale rs = row_scale_bits(top[tid]);
-            scale[tid] = rs.scale;
-            inverse[tid] = rs.inverse;
-        }
-        __syncthreads();
-        for (uint32_t r = 0; r < kRows; ++r) {
-            const RowScale rs{0.0f, inverse[r]};
+            const RowScale rs = row_scale_bits(top[r]);
+            if (tid == 0) scale[r] = rs.scale;
             const P *src = reinterpret_cast<const P *>(a + (size_t)r * p.a_stride);
             for (uint32_t i = tid; i < padded / V; i += kIsThreads) {
                 Q q;
-                if (r < count && i < pieces) {
-                    const P v = src[i];
+                if (i < pieces) {
+                    const P v = r == 0u && i == tid ? early : src[i];
 #pragma unroll
                     for (int x = 0; x < V; ++x) q.v[x] = row_code(elem_to_float(v.v[x]), rs);
                 } else {
@@ -158,10 +183,10 @@ __global__ void __launch_bounds__(kIsThreads) int8_stream_kernel(IsParams p) {
     int acc[NT][4];
 #pragma unroll
     for (int x = 0; x < NT; ++x) acc[x][0] = acc[x][1] = acc[x][2] = acc[x][3] = 0;
-    for (uint32_t s0 = warp; s0 < steps; s0 += kAhead * kIsWarps) {
+    for (uint32_t s0 = part; s0 < steps; s0 += kIsAhead * parts) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t s = s0 + i * kIsWarps;
+        for (uint32_t i = 0; i < kIsAhead; ++i) {
+            const uint32_t s = s0 + i * parts;
             if (s < steps) {
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
@@ -171,7 +196,7 @@ __global__ void __launch_bounds__(kIsThreads) int8_stream_kernel(IsParams p) {
                 }
             }
         }
-        if (s0 + kAhead * kIsWarps < steps) request(s0 + kAhead * kIsWarps);
+        if (s0 + kIsAhead * parts < steps) request(s0 + kIsAhead * parts);
     }
     // the warps' parts of the sums: [warp][tile of 8 rows][lane][4]
 #pragma unroll
@@ -179,22 +204,22 @@ __global__ void __launch_bounds__(kIsThreads) int8_stream_kernel(IsParams p) {
         *reinterpret_cast<int4 *>(partial + ((warp * NT + x) * 32u + lane) * 4u) = make_int4(acc[x][0], acc[x][1], acc[x][2], acc[x][3]);
     __syncthreads();
     // out: consecutive threads take consecutive features of a row
-    constexpr uint32_t kOuts = GATED ? 8u : 16u;
+    const uint32_t across = kFeatures * groups, first = blockIdx.x * across;
     const float *bs = p.b_scales + (size_t)e * p.channels;
-    for (uint32_t i = tid; i < kOuts * kRows; i += kIsThreads) {
-        const uint32_t f = i % kOuts, r = i / kOuts;
-        if (r >= count || j0 + f >= p.n) continue;
+    for (uint32_t i = tid; i < across * count; i += kIsThreads) {
+        const uint32_t r = i / across, f = i - r * across, jf = first + f;
+        if (jf >= p.n) continue;
         // row r is column r % 8 of tile r / 8: lane 4 (f % 8) + (r % 8) / 2, values r % 2 (channel f) and 2 + r % 2 (f + 8)
-        const uint32_t at = ((r / 8u) * 32u + 4u * (f % 8u) + (r % 8u) / 2u) * 4u + (r % 2u) + (!GATED && f >= 8u ? 2u : 0u);
+        const uint32_t in = f % kFeatures;
+        const uint32_t at = ((f / kFeatures * parts * NT + r / 8u) * 32u + 4u * (in % 8u) + (r % 8u) / 2u) * 4u + (r % 2u) + (!GATED && in >= 8u ? 2u : 0u);
         int v = 0, u = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kIsWarps; ++w) {
+        for (uint32_t w = 0; w < parts; ++w) {
             v += partial[w * NT * 128u + at];
             if (GATED) u += partial[w * NT * 128u + at + 2u];
         }
-        float x = (scale[r] * bs[j0 + f]) * (float)v;
-        if (GATED) x = (p.out_elem == ELEM_F32 ? gate_act<false>(x, p.act) : gate_act<true>(x, p.act)) * ((scale[r] * bs[p.n + j0 + f]) * (float)u);
-        store_elem(p.out, p.out_elem, (size_t)(row0 + r) * p.out_stride + j0 + f, x);
+        float x = (scale[r] * bs[jf]) * (float)v;
+        if (GATED) x = (p.out_elem == ELEM_F32 ? gate_act<false>(x, p.act) : gate_act<true>(x, p.act)) * ((scale[r] * bs[p.n + jf]) * (float)u);
+        store_elem(p.out, p.out_elem, (size_t)(row0 + r) * p.out_stride + jf, x);
     }
 }
 

@@ -380,35 +380,59 @@ struct QuantizeParams {
     float *scales;
 };
 
-// A warp per row: the largest magnitude, then the codes (the row comes from the L1 the second time).
-template <typename T, int V>
+// WARPS warps per row, which they hold in registers between the largest magnitude and the codes; a longer row is read twice.
+// 4096 rows of 2048 fp16 elements on a B200: see the table of the documents for times; one row of 2048 takes eight warps 1.9 us,
+// one warp 2.6.
+constexpr int kQuantizeHeld = 8;             // pieces of a row that a lane holds
+template <typename T, int V, int WARPS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p) {
     using P = Piece<T, V>;
     using Q = Piece<int8_t, V>;
+    __shared__ uint32_t top[8];
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t row = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
-    if (row >= p.rows) return;
+    constexpr uint32_t kAcross = 32u * WARPS;
+    const uint32_t warp = threadIdx.x >> 5, in = threadIdx.x % kAcross;
+    const uint32_t row = blockIdx.x * (8u / WARPS) + threadIdx.x / kAcross;
+    if (row >= p.rows) return;               // whole warps, with WARPS = 8 the whole block
     const P *src = reinterpret_cast<const P *>(static_cast<const T *>(p.x) + (size_t)row * p.x_stride);
     Q *dst = reinterpret_cast<Q *>(p.q + (size_t)row * p.q_stride);
-    uint32_t m = 0;
-    constexpr int kUnroll = sizeof(P) == 16 ? 4 : 8;
-#pragma unroll kUnroll
-    for (uint32_t c = lane; c < p.n / V; c += 32u) {
-        const P v = src[c];
+    const uint32_t pieces = p.n / V;
+    auto largest = [](const P &v, uint32_t m) {
 #pragma unroll
         for (int i = 0; i < V; ++i) m = max(m, magnitude_bits(elem_to_float(v.v[i])));
+        return m;
+    };
+    P held[kQuantizeHeld];
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kQuantizeHeld; ++i)
+        if (in + i * kAcross < pieces) held[i] = src[in + i * kAcross];
+#pragma unroll
+    for (uint32_t i = 0; i < kQuantizeHeld; ++i)
+        if (in + i * kAcross < pieces) m = largest(held[i], m);
+#pragma unroll 4
+    for (uint32_t c = in + kQuantizeHeld * kAcross; c < pieces; c += kAcross) m = largest(src[c], m);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (WARPS > 1) {
+        if ((threadIdx.x & 31u) == 0u) top[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WARPS; ++i) m = max(m, top[i]);
     }
-    const RowScale rs = row_scale_bits(__reduce_max_sync(0xffffffffu, m));
-#pragma unroll kUnroll
-    for (uint32_t c = lane; c < p.n / V; c += 32u) {
-        const P v = src[c];
+    const RowScale rs = row_scale_bits(m);
+    auto code = [&](const P &v) {
         Q q;
 #pragma unroll
         for (int i = 0; i < V; ++i) q.v[i] = row_code(elem_to_float(v.v[i]), rs);
-        dst[c] = q;
-    }
-    if (lane == 0) p.scales[row] = rs.scale;
+        return q;
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kQuantizeHeld; ++i)
+        if (in + i * kAcross < pieces) dst[in + i * kAcross] = code(held[i]);
+#pragma unroll 4
+    for (uint32_t c = in + kQuantizeHeld * kAcross; c < pieces; c += kAcross) dst[c] = code(src[c]);
+    if (in == 0u) p.scales[row] = rs.scale;
 }
 
 // ---- launches -------------------------------------------------------------------------------------------
@@ -445,7 +469,11 @@ cudaError_t nvmai::launch_quantize(const void *x, uint32_t elem, uint32_t x_stri
                                    float *scales, cudaStream_t st) {
     const QuantizeParams p{x, x_stride, rows, n, q, q_stride, scales};
     return with_pieces(elem, n, {{x, x_stride, elem_size(elem)}, {q, q_stride, 1}}, [&](auto T, auto V) {
-        return launch_pdl(quantize_rows_kernel<decltype(T), decltype(V)::value>, dim3((rows + 7) / 8), dim3(256), 0, st, true, p);
+        constexpr int v = decltype(V)::value;
+        // A block per row where a warp each would leave SMs with less than eight, or could not hold its row
+        if (rows < 8 * kSms || n > 32u * kQuantizeHeld * v)
+            return launch_pdl(quantize_rows_kernel<decltype(T), v, 8>, dim3(rows), dim3(256), 0, st, true, p);
+        return launch_pdl(quantize_rows_kernel<decltype(T), v, 1>, dim3((rows + 7) / 8), dim3(256), 0, st, true, p);
     });
 }
 
