@@ -467,7 +467,7 @@ NVMAI_API int nvmai_cuda_moe_residual_add_f16(void *hidden, const void *delta, u
  * With x (tokens rows of d elements) and rows it also brings each kept pair's token row to its place;
  * rows behind the last kept one are left as they were.  rows_elem is x_elem (a copy of the bits),
  * or NVMAI_ELEM_I8: codes and row_scales as nvmai_cuda_moe_quantize_rows makes them.  x = rows =
- * NULL: the order alone.  top_k <= 64, num_experts <= 1024, tokens * top_k < 2^31; tokens = 0 is
+ * NULL: the order alone.  top_k <= 64, num_experts <= 1024, tokens * top_k < 2^26; tokens = 0 is
  * valid.  The gradient of x is nvmai_cuda_moe_merge_rows of the rows' gradient, without weights.
  * workspace: device memory, as many bytes as _sort_rows_workspace says (0 for small calls). */
 NVMAI_API uint64_t nvmai_cuda_moe_sort_rows_workspace(uint32_t tokens, uint32_t top_k, uint32_t num_experts);

@@ -20,8 +20,12 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // A stable counting sort: the row of a pair is (kept pairs of smaller experts) + (pairs of its expert in front of it).  Each
 // block has a run of tokens; it counts the experts of all pairs, those in front of its run apart, and ranks its own pairs
 // with one warp, 32 at a time (__match_any_sync gives the pairs of the same expert).  Then its warps move the tokens' rows.
-constexpr int kSortThreads = 1024;
+constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kSms = 148, kSortBlocks = kSms;
+constexpr uint32_t kSortOwn = 4096;          // most pairs of a block: their experts and rows are in shared memory
+// From this many pairs on the blocks' counts come from a kernel in front (the order alone on a B200, top-8 of 256: 8192 tokens 10.3
+// us with all pairs counted by every block, 9.4 with that kernel; 16384 tokens 18.0 / 13.3; 65536 tokens 57 / 28).
+constexpr uint32_t kSortCounted = 65536;
 
 struct SortParams {
     const uint32_t *idx; uint32_t tokens, top_k, E;
@@ -29,7 +33,30 @@ struct SortParams {
     const void *x; size_t x_stride; uint32_t d;
     void *rows; size_t rows_stride;
     float *row_scales;
+    uint32_t *counts;        // [blocks][sort_columns(E)], or nullptr: every block counts all pairs
 };
+__host__ __device__ constexpr uint32_t sort_columns(uint32_t E) { return (E + 3u) & ~3u; }
+
+__device__ __forceinline__ uint32_t sort_first_token(const SortParams &p, uint32_t block) {
+    return (uint32_t)((uint64_t)p.tokens * block / gridDim.x);
+}
+
+// Kept pairs of each expert in a block's run.
+__global__ void __launch_bounds__(512) sort_count_kernel(SortParams p) {
+    __shared__ uint32_t count[kRowMaxExperts];
+    const uint32_t lo = sort_first_token(p, blockIdx.x) * p.top_k, hi = sort_first_token(p, blockIdx.x + 1) * p.top_k;
+    const uint32_t columns = sort_columns(p.E);
+    for (uint32_t e = threadIdx.x; e < columns; e += blockDim.x) count[e] = 0u;
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
+    for (uint32_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+        const uint32_t e = p.idx[i];
+        if (e < p.E) atomicAdd(&count[e], 1u);
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < columns; e += blockDim.x) p.counts[(size_t)blockIdx.x * columns + e] = count[e];
+}
 
 // sum over the threads in front of this one (1024 threads); *total gets the sum over all
 __device__ __forceinline__ uint32_t block_exclusive_sum(uint32_t v, uint32_t *warp_sums, uint32_t *total) {
@@ -59,18 +86,42 @@ __device__ __forceinline__ uint32_t block_exclusive_sum(uint32_t v, uint32_t *wa
 // MOVE: 0 the order alone, 1 rows as they are, 2 as codes.  T: what a row is read as (MOVE 1: bits of that size), V at a time.
 template <typename T, int V, int MOVE>
 __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
+    using P = Piece<T, V>;
+    using Q = Piece<int8_t, V>;
     __shared__ uint32_t before[kRowMaxExperts + 1], rest[kRowMaxExperts + 1], warp_sums[32];
+    __shared__ uint32_t own[kSortOwn], unkept;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const uint32_t first = (uint32_t)((uint64_t)p.tokens * blockIdx.x / gridDim.x);
-    const uint32_t last = (uint32_t)((uint64_t)p.tokens * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t first = sort_first_token(p, blockIdx.x), last = sort_first_token(p, blockIdx.x + 1);
     const uint32_t pairs = p.tokens * p.top_k, lo = first * p.top_k, hi = last * p.top_k;
     for (uint32_t e = tid; e <= p.E; e += kSortThreads) before[e] = rest[e] = 0u;
+    if (tid == 0) unkept = lo;
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    for (uint32_t i = tid; i < pairs; i += kSortThreads) {
-        const uint32_t e = min(p.idx[i], p.E);
-        atomicAdd(i < lo ? &before[e] : &rest[e], 1u);
+    for (uint32_t i = lo + tid; i < hi; i += kSortThreads) own[i - lo] = min(p.idx[i], p.E);
+    if (p.counts == nullptr) {
+#pragma unroll 4
+        for (uint32_t i = tid; i < pairs; i += kSortThreads) {
+            const uint32_t e = min(p.idx[i], p.E);
+            atomicAdd(i < lo ? &before[e] : &rest[e], 1u);
+        }
+    } else {
+        // 128 neighbouring experts a warp, the blocks spread over the warps that share them
+        const uint32_t columns = sort_columns(p.E), across = (columns + 127u) / 128u, shares = kSortWarps / across;
+        const uint32_t e = warp % across * 128u + lane * 4u;
+        if (warp < across * shares && e < columns) {
+            uint4 in_front = make_uint4(0, 0, 0, 0), behind = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+            for (uint32_t b = warp / across; b < gridDim.x; b += shares) {
+                const uint4 n = *reinterpret_cast<const uint4 *>(p.counts + (size_t)b * columns + e);
+                if (b < blockIdx.x) { in_front.x += n.x; in_front.y += n.y; in_front.z += n.z; in_front.w += n.w; }
+                else { behind.x += n.x; behind.y += n.y; behind.z += n.z; behind.w += n.w; }
+            }
+            const uint32_t f[4] = {in_front.x, in_front.y, in_front.z, in_front.w}, r[4] = {behind.x, behind.y, behind.z, behind.w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+                if (e + i < p.E) { atomicAdd(&before[e + i], f[i]); atomicAdd(&rest[e + i], r[i]); }
+        }
     }
     __syncthreads();
     const uint32_t ahead = tid < p.E ? before[tid] : 0u;
@@ -80,55 +131,66 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
         before[tid] = base + ahead;              // row of the next pair of this expert
         if (blockIdx.x == 0) p.begin[tid] = base;
     }
-    if (tid == 0) {
-        before[p.E] += kept;                     // pairs that are not kept name the rows behind
-        if (blockIdx.x == 0) p.begin[p.E] = kept;
-    }
+    if (tid == 0 && blockIdx.x == 0) p.begin[p.E] = kept;
+    // pairs that are not kept name the rows behind: those in front of the run are lo less the kept ones in front of it
+    const uint32_t kept_ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if (lane == 0) atomicSub(&unkept, kept_ahead);
+    __syncthreads();
+    if (tid == 0) before[p.E] = unkept + kept;
     __syncthreads();
     if (warp == 0) {
         for (uint32_t i0 = lo; i0 < hi; i0 += 32u) {
             const uint32_t i = i0 + lane;
-            const uint32_t e = i < hi ? min(p.idx[i], p.E) : 0xFFFFFFFFu;
+            const uint32_t e = i < hi ? own[i - lo] : 0xFFFFFFFFu;
             const uint32_t same = __match_any_sync(0xffffffffu, e);
             uint32_t row = 0;
             if (i < hi) row = before[e] + __popc(same & ((1u << lane) - 1u));
             __syncwarp();
             if (i < hi) {
                 if ((same >> lane) == 1u) before[e] = row + 1u;          // the last of them
+                const uint32_t at = e < p.E ? row : kNoRow;
                 p.source[row] = e < p.E ? i : kNoRow;
-                p.position[i] = e < p.E ? row : kNoRow;
+                p.position[i] = at;
+                own[i - lo] = at;
             }
             __syncwarp();
         }
     }
     if constexpr (MOVE != 0) {
         __syncthreads();
+        auto code = [](const P &v, const RowScale &rs) {
+            Q q;
+#pragma unroll
+            for (int x = 0; x < V; ++x) q.v[x] = row_code(elem_to_float(v.v[x]), rs);
+            return q;
+        };
+        auto scale_out = [&](const uint32_t *place, float scale) {
+            for (uint32_t k = lane; k < p.top_k; k += 32u)
+                if (place[k] != kNoRow) p.row_scales[place[k]] = scale;
+        };
         // a warp takes a token's row, or a part of it where the block has fewer tokens than warps
-        const uint32_t mine = last - first, warps = kSortThreads / 32;
-        const uint32_t parts = mine == 0 || mine >= warps ? 1u : warps / mine;
+        const uint32_t mine = last - first;
+        const uint32_t parts = mine == 0 || mine >= kSortWarps ? 1u : kSortWarps / mine;
         const uint32_t pieces = p.d / V, each = (pieces + parts - 1u) / parts;
-        for (uint32_t u = warp; u < mine * parts; u += warps) {
+        for (uint32_t u = warp; u < mine * parts; u += kSortWarps) {
             const uint32_t t = first + u / parts, part = u % parts;
             const uint32_t c0 = part * each, c1 = min(pieces, c0 + each);
-            const T *src = static_cast<const T *>(p.x) + (size_t)t * p.x_stride;
-            const uint32_t *pos = p.position + (size_t)t * p.top_k;
+            const P *src = reinterpret_cast<const P *>(static_cast<const T *>(p.x) + (size_t)t * p.x_stride);
+            const uint32_t *place = own + (t - first) * p.top_k;
             if constexpr (MOVE == 1) {
-                using P = Piece<T, V>;
 #pragma unroll 4
                 for (uint32_t c = c0 + lane; c < c1; c += 32u) {
-                    const P v = reinterpret_cast<const P *>(src)[c];
+                    const P v = src[c];
                     for (uint32_t k = 0; k < p.top_k; ++k) {
-                        const uint32_t row = pos[k];
+                        const uint32_t row = place[k];
                         if (row != kNoRow) reinterpret_cast<P *>(static_cast<T *>(p.rows) + (size_t)row * p.rows_stride)[c] = v;
                     }
                 }
             } else {
-                using P = Piece<T, V>;
-                using Q = Piece<int8_t, V>;
                 uint32_t m = 0;
 #pragma unroll 4
                 for (uint32_t c = lane; c < pieces; c += 32u) {
-                    const P v = reinterpret_cast<const P *>(src)[c];
+                    const P v = src[c];
 #pragma unroll
                     for (int i = 0; i < V; ++i) m = max(m, magnitude_bits(elem_to_float(v.v[i])));
                 }
@@ -136,18 +198,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
                 const RowScale rs = row_scale_bits(m);
 #pragma unroll 4
                 for (uint32_t c = c0 + lane; c < c1; c += 32u) {
-                    const P v = reinterpret_cast<const P *>(src)[c];
-                    Q q;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) q.v[i] = row_code(elem_to_float(v.v[i]), rs);
+                    const Q q = code(src[c], rs);
                     for (uint32_t k = 0; k < p.top_k; ++k) {
-                        const uint32_t row = pos[k];
+                        const uint32_t row = place[k];
                         if (row != kNoRow) reinterpret_cast<Q *>(static_cast<int8_t *>(p.rows) + (size_t)row * p.rows_stride)[c] = q;
                     }
                 }
-                if (part == 0)
-                    for (uint32_t k = lane; k < p.top_k; k += 32u)
-                        if (pos[k] != kNoRow) p.row_scales[pos[k]] = rs.scale;
+                if (part == 0) scale_out(place, rs.scale);
             }
         }
     }
@@ -477,9 +534,18 @@ cudaError_t nvmai::launch_quantize(const void *x, uint32_t elem, uint32_t x_stri
     });
 }
 
+// every block has at least a token and at most kSortOwn pairs
+static uint32_t sort_blocks(uint32_t tokens, uint32_t top_k) {
+    const uint32_t most = kSortOwn / top_k;
+    return std::max({1u, std::min(tokens, kSortBlocks), (uint32_t)(((uint64_t)tokens + most - 1) / most)});
+}
+
 extern "C" {
 
-uint64_t nvmai_cuda_moe_sort_rows_workspace(uint32_t, uint32_t, uint32_t) { return 0; }
+uint64_t nvmai_cuda_moe_sort_rows_workspace(uint32_t tokens, uint32_t top_k, uint32_t num_experts) {
+    if ((uint64_t)tokens * top_k < kSortCounted || top_k > kRowMaxTopK) return 0;
+    return (uint64_t)sort_blocks(tokens, top_k) * sort_columns(num_experts) * 4;
+}
 
 int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_k, uint32_t num_experts, uint32_t *position,
                              uint32_t *source, uint32_t *expert_begin, const void *x, uint32_t x_elem, uint32_t x_stride, uint32_t d,
@@ -487,7 +553,7 @@ int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_
                              uint64_t workspace_bytes, void *stream) {
     if (!expert_begin || (tokens != 0 && (!idx || !position || !source))) return NVMAI_CUDA_EINVAL;
     if (top_k == 0 || top_k > kRowMaxTopK || num_experts == 0 || num_experts > kRowMaxExperts) return NVMAI_CUDA_ERANGE;
-    if ((uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+    if ((uint64_t)tokens * top_k >= (1ull << 26)) return NVMAI_CUDA_ERANGE;
     if (!aligned_to(idx, 4) || !aligned_to(position, 4) || !aligned_to(source, 4) || !aligned_to(expert_begin, 4)) return NVMAI_CUDA_EINVAL;
     if ((x == nullptr) != (rows == nullptr)) return NVMAI_CUDA_EINVAL;
     if (x != nullptr) {
@@ -496,11 +562,16 @@ int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_
         if (!aligned_to(x, elem_size(x_elem)) || !aligned_to(rows, elem_size(rows_elem))) return NVMAI_CUDA_EINVAL;
         if ((rows_elem == ELEM_I8) != (row_scales != nullptr) || !aligned_to(row_scales, 4)) return NVMAI_CUDA_EINVAL;
     }
-    if (workspace_bytes < nvmai_cuda_moe_sort_rows_workspace(tokens, top_k, num_experts)) return NVMAI_CUDA_ERANGE;
-    if (!on_current_device({idx, position, source, expert_begin, x, rows, row_scales})) return NVMAI_CUDA_EINVAL;
-    const SortParams p{idx, tokens, top_k, num_experts, position, source, expert_begin, x, x_stride, d, rows, rows_stride, row_scales};
-    const dim3 grid(std::max(1u, std::min(tokens, kSortBlocks))), block(kSortThreads);
+    const uint64_t counts_bytes = nvmai_cuda_moe_sort_rows_workspace(tokens, top_k, num_experts);
+    if (workspace_bytes < counts_bytes) return NVMAI_CUDA_ERANGE;
+    if (counts_bytes != 0 && (!workspace || !aligned_to(workspace, 16))) return NVMAI_CUDA_EINVAL;
+    if (!on_current_device({idx, position, source, expert_begin, x, rows, row_scales, counts_bytes != 0 ? workspace : nullptr})) return NVMAI_CUDA_EINVAL;
+    const SortParams p{idx, tokens, top_k, num_experts, position, source, expert_begin, x, x_stride, d, rows, rows_stride, row_scales,
+                       counts_bytes != 0 ? static_cast<uint32_t *>(workspace) : nullptr};
+    const dim3 grid(sort_blocks(tokens, top_k)), block(kSortThreads);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.counts != nullptr)
+        if (const int rc = launched(launch_pdl(sort_count_kernel, grid, dim3(512), 0, st, true, p))) return rc;
     if (x == nullptr) return launched(launch_pdl(sort_rows_kernel<float, 1, 0>, grid, block, 0, st, true, p));
     return with_pieces(x_elem, d, {{x, x_stride, elem_size(x_elem)}, {rows, rows_stride, elem_size(rows_elem)}}, [&](auto T, auto V) {
         constexpr int v = decltype(V)::value;

@@ -37,6 +37,10 @@ E, R = _lib.EINVAL, _lib.ERANGE
     ("sort_rows", SORT, dict(num_experts=0), R),
     ("sort_rows", SORT, dict(num_experts=1025), R),
     ("sort_rows", SORT, dict(tokens=1 << 30), R),
+    ("sort_rows", SORT, dict(tokens=1 << 25), R),
+    ("sort_rows", SORT, dict(tokens=1 << 24), R),                             # without its workspace
+    ("sort_rows", SORT, dict(tokens=1 << 24, workspace_bytes=1 << 40), E),
+    ("sort_rows", SORT, dict(tokens=1 << 24, workspace=A + 8, workspace_bytes=1 << 40), E),
     ("sort_rows", SORT, dict(x=None), E),
     ("sort_rows", SORT, dict(rows=None), E),
     ("sort_rows", SORT, dict(d=0), E),
@@ -124,8 +128,11 @@ def test_nothing_to_do_is_no_error(lib, name, good, change):
     assert getattr(lib, "nvmai_cuda_moe_" + name)(*{**good, **change}.values()) == _lib.OK
 
 
-def test_workspaces_hold_codes_and_scales():
-    from nvmai_b200 import int8_matmul_workspace
+def test_workspaces_hold_counts_codes_and_scales():
+    from nvmai_b200 import int8_matmul_workspace, sort_rows_workspace
+    assert sort_rows_workspace(4096, 8, 256) == 0
+    assert sort_rows_workspace(16384, 8, 256) == 148 * 256 * 4
+    assert sort_rows_workspace(1 << 20, 8, 1024) == 2048 * 1024 * 4          # a block's pairs stay 4096
     assert int8_matmul_workspace(77, 100, fmt.ELEM_I8) == 0
     for elem in (fmt.ELEM_F16, fmt.ELEM_F32, fmt.ELEM_BF16):
         assert int8_matmul_workspace(77, 100, elem) >= 77 * 112 + 77 * 4
