@@ -310,38 +310,47 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
                 for (uint32_t c = 0; c < 16u; ++c, o += p.out_stride)
                     if (mine && c < live) *o = elem_from_float<OUT>(x[c]);
             };
-            for (uint32_t i = 0, c0 = part * 16u; c0 < un.count; ++i, c0 += 64u) {
-                OUT *out = static_cast<OUT *>(p.out) + (size_t)(un.row + c0) * p.out_stride + j0;
-                const uint32_t live = un.count - c0;
-                float x[16];
-                uint32_t v[16];
-                if constexpr (GATED) {
-                    uint32_t v1[16];
-                    tmem_ld16(acc + c0, v);
-                    tmem_ld16(acc + p.nt + c0, v1);
-                    tmem_ld_wait();
+            // Some runs at a time: the accumulators are free for the next unit's MMAs as soon as the last ones are in registers, not when
+            // they are stored.
+            constexpr uint32_t kRuns = GATED ? 2 : 2 / SUBS;
+            for (uint32_t i = 0;; i += kRuns) {
+                const uint32_t c0 = (part + 4u * i) * 16u;
+                uint32_t v[kRuns][SUBS][16];
 #pragma unroll
-                    for (uint32_t c = 0; c < 16u; ++c) {
-                        const float sa = reinterpret_cast<const float *>(scales)[i * 16u + c];
-                        x[c] = gate_act<kHalf>((sa * sb0) * (float)(int)v[c], p.act) * ((sa * sb1) * (float)(int)v1[c]);
-                    }
-                    store(x, out, live, live0);
-                } else {
+                for (uint32_t r = 0; r < kRuns; ++r)
+                    if (c0 + 64u * r < un.count)
 #pragma unroll
-                    for (uint32_t t = 0; t < SUBS; ++t) {
-                        tmem_ld16(acc + t * p.nt + c0, v);
-                        tmem_ld_wait();
-                        const float sb = t ? sb1 : sb0;
+                        for (uint32_t t = 0; t < SUBS; ++t) tmem_ld16(acc + t * p.nt + c0 + 64u * r, v[r][t]);
+                tmem_ld_wait();
+                if (c0 + 64u * kRuns >= un.count) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s.acc_empty[buf]);
+                }
 #pragma unroll
-                        for (uint32_t c = 0; c < 16u; ++c)
-                            x[c] = (reinterpret_cast<const float *>(scales)[i * 16u + c] * sb) * (float)(int)v[c];
-                        store(x, out + 128u * t, live, t ? live1 : live0);
+                for (uint32_t r = 0; r < kRuns; ++r) {
+                    const uint32_t c = c0 + 64u * r;
+                    if (c >= un.count) break;
+                    OUT *out = static_cast<OUT *>(p.out) + (size_t)(un.row + c) * p.out_stride + j0;
+                    const float *sa = reinterpret_cast<const float *>(scales) + (i + r) * 16u;
+                    float x[16];
+                    if constexpr (GATED) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 16u; ++k)
+                            x[k] = gate_act<kHalf>((sa[k] * sb0) * (float)(int)v[r][0][k], p.act) * ((sa[k] * sb1) * (float)(int)v[r][1][k]);
+                        store(x, out, un.count - c, live0);
+                    } else {
+#pragma unroll
+                        for (uint32_t t = 0; t < SUBS; ++t) {
+#pragma unroll
+                            for (uint32_t k = 0; k < 16u; ++k) x[k] = (sa[k] * (t ? sb1 : sb0)) * (float)(int)v[r][t][k];
+                            store(x, out + 128u * t, un.count - c, t ? live1 : live0);
+                        }
                     }
                 }
+                if (c0 + 64u * kRuns >= un.count) break;
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.acc_empty[buf]);
+            __syncwarp();                                          // before the next unit's scales
         }
     }
     __syncwarp();
