@@ -454,9 +454,10 @@ NVMAI_API int nvmai_cuda_moe_residual_add_f16(void *hidden, const void *delta, u
  * in the reference.  No handle: every buffer is the caller's, nothing is allocated, no state is
  * kept between calls, and calls on different streams are independent as long as their buffers
  * (workspaces included) are.  Calls can be captured.  Strides count elements (codes: bytes) from
- * one row to the next and are at least the row's length.  All pointers belong to the current
- * device (NVMAI_CUDA_EINVAL otherwise); indexes and positions are checked on the device, an
- * entry out of range counts as not held, never as an address. */
+ * one row to the next and are at least the row's length.  All pointers are memory of the current
+ * device, or managed memory (NVMAI_CUDA_EINVAL otherwise); indexes and positions are checked on
+ * the device, an entry out of range counts as not held, never as an address.  Outputs overlap
+ * neither inputs nor each other, except where a call says so. */
 
 /* Sorts the tokens * top_k pairs (token t, slot k), pair = t * top_k + k, by expert: pairs with
  * idx[pair] < num_experts are kept, ordered by (expert, pair); the others (a padded row's, another
@@ -512,8 +513,8 @@ NVMAI_API int nvmai_cuda_moe_quantize_rows(const void *x, uint32_t elem, uint32_
  * a: codes with a_scales (NVMAI_ELEM_I8), or F16 / F32 / BF16 rows with a_scales = NULL, which the call
  * quantises as quantize_rows does; these need a workspace of _int8_matmul_workspace bytes.
  * Codes start on 16-byte boundaries and their strides are multiples of 16.  k < 131072 (the sum fits 32 bits);
- * rows = 0 is valid.  Without an explicit wait of its own the call cannot report a device-side wait that gave up:
- * nvmai_cuda_moe_int8_matmul_status does. */
+ * rows = 0 is valid.  The bits of a row's output do not depend on the rows beside it.  A bounded
+ * device-side wait that gives up is reported by nvmai_cuda_moe_int8_matmul_status. */
 NVMAI_API uint64_t nvmai_cuda_moe_int8_matmul_workspace(uint32_t rows, uint32_t k, uint32_t a_elem);
 NVMAI_API int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride, const float *a_scales,
                                          uint32_t rows, uint32_t k, const void *b, uint32_t b_stride,
@@ -522,8 +523,13 @@ NVMAI_API int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_
                                          uint32_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream);
 
 /* Waits for `stream`, then returns NVMAI_CUDA_ETIMEOUT if a bounded device-side wait of an int8_matmul call on the
- * current device gave up since the last call of this function (the outputs of that product are undefined), else 0. */
+ * current device gave up since the last call of this function (the outputs of that product are undefined), else 0.
+ * NVMAI_CUDA_EINVAL on a stream that is being captured. */
 NVMAI_API int nvmai_cuda_moe_int8_matmul_status(void *stream);
+
+/* Test hook for that failure path: the next int8_matmul call that runs on the tcgen05 kernel (more than 32 rows) with
+ * k > 128 leaves out one copy, so its bounded waits run out.  Nothing faults or hangs. */
+NVMAI_API int nvmai_cuda_moe_debug_drop_int8_copy(void);
 
 /* Optional per-kernel timeline of the single-token decode stages, the counterpart
  * of the reference's NVMAI_KERNEL_STATS command-buffer times

@@ -92,6 +92,7 @@ PROTOTYPES = {
     "nvmai_cuda_moe_int8_matmul_workspace": (u64, [u32, u32, u32]),
     "nvmai_cuda_moe_int8_matmul": (C.c_int, [vp, u32, u32, vp, u32, u32, vp, u32, vp, u32, u32, vp, u32, vp, u32, u32, vp, u64, vp]),
     "nvmai_cuda_moe_int8_matmul_status": (C.c_int, [vp]),
+    "nvmai_cuda_moe_debug_drop_int8_copy": (C.c_int, []),
     "nvmai_cuda_moe_set_trace": (C.c_int, [vp, C.c_int]),
     "nvmai_cuda_moe_read_trace": (C.c_int, [vp, vp, u32]),
     "nvmai_cuda_moe_read_block_trace": (C.c_int, [vp, vp, u32, C.POINTER(u32)]),

@@ -30,6 +30,7 @@ struct IgParams {
     uint32_t paired;                     // 16-bit outputs: two neighbouring channels go out in one store
     uint32_t channel_tiles;              // units across the channels
     unsigned int *status;
+    uint32_t debug_drop_rows;            // test hook: block 0 leaves out the rows of its second K block, so waits run out
 };
 struct alignas(64) IgArgs {
     CUtensorMap a, b;                    // [rows][k], [E * channels][k] bytes; boxes of 32 and of 128 rows x 128 bytes
@@ -221,17 +222,18 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
                         if (!(ok = wait(&s.empty[stage], parity))) break;
                         load_channels(un, kb, stage);
                     }
-                    for (uint32_t i = 0; i < boxes; ++i)
+                    const bool drop = p.debug_drop_rows != 0u && u == 0u && kb == 1u;
+                    for (uint32_t i = 0; i < boxes && !drop; ++i)
                         tma_load_2d(slot + SUBS * kIgTileBytes + i * kIgBoxRows * 128u, &args.a, kb * 128u, un.row + i * kIgBoxRows, &s.full[stage]);
                     ++filled;
                     if (++stage == p.stages) { stage = 0; parity ^= 1u; }
                 }
             }
             if (!ok) {      // copies in flight end before the block does
-                const unsigned long long t0 = global_timer_ns();
+                const unsigned long long t0 = global_timer_ns(), limit = g_wait_limit_ns;
                 for (uint32_t i = 0; i < min(filled, p.stages); ++i) {
                     const uint32_t at = (stage + p.stages - 1u - i) % p.stages, lap = (filled - 1u - i) / p.stages;
-                    while (!mbar_try_wait_short(&s.full[at], lap & 1u) && global_timer_ns() - t0 < 1000000000ull) {}
+                    while (!mbar_try_wait_short(&s.full[at], lap & 1u) && global_timer_ns() - t0 < limit) {}
                 }
             }
         }
@@ -263,8 +265,8 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
             }
             if (!ok) {      // MMAs in flight end before their operands and accumulators go
                 umma_commit(&s.drained);
-                const unsigned long long t0 = global_timer_ns();
-                while (!mbar_try_wait_short(&s.drained, 0u) && global_timer_ns() - t0 < 1000000000ull) {}
+                const unsigned long long t0 = global_timer_ns(), limit = g_wait_limit_ns;
+                while (!mbar_try_wait_short(&s.drained, 0u) && global_timer_ns() - t0 < limit) {}
             }
         }
     } else {

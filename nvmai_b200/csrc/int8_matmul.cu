@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -48,17 +49,21 @@ bool code_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t k, uin
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The status word's address on the current device.
 unsigned int *status_word() {
-    static unsigned int *at[64] = {};
+    static std::atomic<unsigned int *> at[64] = {};
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    if (at[dev] == nullptr) {
+    unsigned int *known = at[dev].load(std::memory_order_acquire);
+    if (known == nullptr) {
         void *p = nullptr;
         if (cudaGetSymbolAddress(&p, g_int8_status) != cudaSuccess) { cudaGetLastError(); return nullptr; }
-        at[dev] = static_cast<unsigned int *>(p);
+        known = static_cast<unsigned int *>(p);
+        at[dev].store(known, std::memory_order_release);
     }
-    return at[dev];
+    return known;
 }
+std::atomic<bool> g_drop_copy{false};      // test hook, see nvmai_cuda_moe_debug_drop_int8_copy
 
 constexpr uint32_t kSms = 148;
 
@@ -114,6 +119,7 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     const size_t stage = subs * kIgTileBytes + (size_t)p.nt * 128;
     p.accs = 2 * subs * p.nt <= 512 ? 2 : 1;
     p.ready = m.ready;
+    p.debug_drop_rows = g_drop_copy.exchange(false) ? 1 : 0;
     p.paired = m.n % 2 == 0 && m.out_stride % 2 == 0 && aligned_to(m.out, 4);
     p.stages = (uint32_t)std::min<size_t>(kIgMaxStages, (227 * 1024 - sizeof(IgShared) - 2048) / stage);
     const size_t smem = 1024 + p.stages * stage;
@@ -170,6 +176,8 @@ cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
 
 }  // namespace
 
+cudaError_t nvmai::int8_set_wait_limit(unsigned long long ns) { return cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns)); }
+
 extern "C" {
 
 uint64_t nvmai_cuda_moe_int8_matmul_workspace(uint32_t rows, uint32_t k, uint32_t a_elem) {
@@ -180,45 +188,50 @@ int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride
                                const void *b, uint32_t b_stride, const float *b_scales, uint32_t n, uint32_t num_experts,
                                const uint32_t *expert_begin, uint32_t activation, void *out, uint32_t out_elem, uint32_t out_stride,
                                void *workspace, uint64_t workspace_bytes, void *stream) {
-    if (!b || !b_scales || (rows != 0 && (!a || !out))) return NVMAI_CUDA_EINVAL;
-    if (a_elem > ELEM_I8 || out_elem > ELEM_BF16 || activation > NVMAI_ACT_NONE) return NVMAI_CUDA_EINVAL;
-    if (k == 0 || n == 0 || a_stride < k || b_stride < k || out_stride < n) return NVMAI_CUDA_EINVAL;
-    if (num_experts == 0 || (!expert_begin && num_experts != 1)) return NVMAI_CUDA_EINVAL;
-    const uint64_t channels = activation == NVMAI_ACT_NONE ? n : 2ull * n;
-    if (k >= 131072 || num_experts > kRowMaxExperts || rows >= (1u << 31) || channels * num_experts >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
-    if (!aligned_to(b, 16) || b_stride % 16 != 0 || !aligned_to(b_scales, 4) || !aligned_to(out, elem_size(out_elem)) || !aligned_to(expert_begin, 4))
-        return NVMAI_CUDA_EINVAL;
-    const bool coded = a_elem == ELEM_I8;
-    if (coded != (a_scales != nullptr) && rows != 0) return NVMAI_CUDA_EINVAL;
-    if (coded ? !aligned_to(a, 16) || a_stride % 16 != 0 || !aligned_to(a_scales, 4) : !aligned_to(a, elem_size(a_elem))) return NVMAI_CUDA_EINVAL;
-    if (rows == 0) return NVMAI_CUDA_OK;
-    if (!coded) {
-        if (workspace_bytes < nvmai_cuda_moe_int8_matmul_workspace(rows, k, a_elem)) return NVMAI_CUDA_ERANGE;
-        if (!workspace || !aligned_to(workspace, 16)) return NVMAI_CUDA_EINVAL;
-    }
-    if (!on_current_device({a, a_scales, b, b_scales, expert_begin, out, coded ? nullptr : workspace})) return NVMAI_CUDA_EINVAL;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    Matmul m{a, a_elem, a_stride, a_scales, rows, k, static_cast<const int8_t *>(b), b_stride, b_scales, n, (uint32_t)channels,
-             num_experts, expert_begin, activation, out, out_elem, out_stride, false};
-    auto launched = [](cudaError_t e) {
-        count_launches(1);
-        if (e != cudaSuccess) cudaGetLastError();
-        return e == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
-    };
-    const uint32_t nt = stream_tiles(m);
-    if (!coded && !(nt && stream_quantizes(m))) {
-        int8_t *q = static_cast<int8_t *>(workspace);
-        float *scales = reinterpret_cast<float *>(q + scales_offset(rows, k));
-        const int rc = launched(launch_quantize(a, a_elem, a_stride, rows, k, q, (uint32_t)code_stride(k), scales, st));
-        if (rc) return rc;
-        m.a = q; m.a_elem = ELEM_I8; m.a_stride = code_stride(k); m.a_scales = scales; m.ready = true;
-    }
-    return launched(nt ? launch_stream(m, nt, st) : launch_gemm(m, st));
+    return without_exceptions([&]() -> int {
+        if (!b || !b_scales || (rows != 0 && (!a || !out))) return NVMAI_CUDA_EINVAL;
+        if (a_elem > ELEM_I8 || out_elem > ELEM_BF16 || activation > NVMAI_ACT_NONE) return NVMAI_CUDA_EINVAL;
+        if (k == 0 || n == 0 || a_stride < k || b_stride < k || out_stride < n) return NVMAI_CUDA_EINVAL;
+        if (num_experts == 0 || (!expert_begin && num_experts != 1)) return NVMAI_CUDA_EINVAL;
+        const uint64_t channels = activation == NVMAI_ACT_NONE ? n : 2ull * n;
+        if (k >= 131072 || num_experts > kRowMaxExperts || rows >= (1u << 31) || channels * num_experts >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+        if (!aligned_to(b, 16) || b_stride % 16 != 0 || !aligned_to(b_scales, 4) || !aligned_to(out, elem_size(out_elem)) || !aligned_to(expert_begin, 4))
+            return NVMAI_CUDA_EINVAL;
+        const bool coded = a_elem == ELEM_I8;
+        if (coded != (a_scales != nullptr) && rows != 0) return NVMAI_CUDA_EINVAL;
+        if (coded ? !aligned_to(a, 16) || a_stride % 16 != 0 || !aligned_to(a_scales, 4) : !aligned_to(a, elem_size(a_elem))) return NVMAI_CUDA_EINVAL;
+        if (rows == 0) return NVMAI_CUDA_OK;
+        if (!coded) {
+            if (workspace_bytes < nvmai_cuda_moe_int8_matmul_workspace(rows, k, a_elem)) return NVMAI_CUDA_ERANGE;
+            if (!workspace || !aligned_to(workspace, 16)) return NVMAI_CUDA_EINVAL;
+        }
+        if (!on_current_device({a, a_scales, b, b_scales, expert_begin, out, coded ? nullptr : workspace})) return NVMAI_CUDA_EINVAL;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        Matmul m{a, a_elem, a_stride, a_scales, rows, k, static_cast<const int8_t *>(b), b_stride, b_scales, n, (uint32_t)channels,
+                 num_experts, expert_begin, activation, out, out_elem, out_stride, false};
+        auto launched = [](cudaError_t e) {
+            count_launches(1);
+            if (e != cudaSuccess) cudaGetLastError();
+            return e == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
+        };
+        const uint32_t nt = stream_tiles(m);
+        if (!coded && !(nt && stream_quantizes(m))) {
+            int8_t *q = static_cast<int8_t *>(workspace);
+            float *scales = reinterpret_cast<float *>(q + scales_offset(rows, k));
+            const int rc = launched(launch_quantize(a, a_elem, a_stride, rows, k, q, (uint32_t)code_stride(k), scales, st));
+            if (rc) return rc;
+            m.a = q; m.a_elem = ELEM_I8; m.a_stride = code_stride(k); m.a_scales = scales; m.ready = true;
+        }
+        return launched(nt ? launch_stream(m, nt, st) : launch_gemm(m, st));
+    });
 }
 
 int nvmai_cuda_moe_int8_matmul_status(void *stream) {
     unsigned int status = 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &capturing) != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
+    if (capturing != cudaStreamCaptureStatusNone) return NVMAI_CUDA_EINVAL;        // a capture has nothing to wait for
     if (cudaMemcpyFromSymbolAsync(&status, g_int8_status, sizeof(status), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
         cudaStreamSynchronize(st) != cudaSuccess) {
         cudaGetLastError();
@@ -231,6 +244,11 @@ int nvmai_cuda_moe_int8_matmul_status(void *stream) {
         return NVMAI_CUDA_ECUDA;
     }
     return NVMAI_CUDA_ETIMEOUT;
+}
+
+int nvmai_cuda_moe_debug_drop_int8_copy(void) {
+    g_drop_copy.store(true);
+    return NVMAI_CUDA_OK;
 }
 
 }  // extern "C"

@@ -33,6 +33,7 @@
 #include "misc_kernels.cuh"
 #include "persistent_batch.cuh"
 #include "persistent_decode.cuh"
+#include "row_ops.h"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
 
@@ -2571,7 +2572,7 @@ int nvmai_cuda_moe_debug_mute_block(nvmai_cuda_moe *h, uint32_t block) {
 
 int nvmai_cuda_moe_debug_set_wait_limit(uint64_t nanoseconds) {
     const unsigned long long v = nanoseconds ? nanoseconds : 1000000000ull;
-    if (bp_set_wait_limit(v) != cudaSuccess) return NVMAI_CUDA_ECUDA;
+    if (bp_set_wait_limit(v) != cudaSuccess || int8_set_wait_limit(v) != cudaSuccess) return NVMAI_CUDA_ECUDA;
     return cudaMemcpyToSymbol(g_wait_limit_ns, &v, sizeof(v)) == cudaSuccess ? NVMAI_CUDA_OK : NVMAI_CUDA_ECUDA;
 }
 

@@ -551,106 +551,114 @@ int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_
                              uint32_t *source, uint32_t *expert_begin, const void *x, uint32_t x_elem, uint32_t x_stride, uint32_t d,
                              void *rows, uint32_t rows_elem, uint32_t rows_stride, float *row_scales, void *workspace,
                              uint64_t workspace_bytes, void *stream) {
-    if (!expert_begin || (tokens != 0 && (!idx || !position || !source))) return NVMAI_CUDA_EINVAL;
-    if (top_k == 0 || top_k > kRowMaxTopK || num_experts == 0 || num_experts > kRowMaxExperts) return NVMAI_CUDA_ERANGE;
-    if ((uint64_t)tokens * top_k >= (1ull << 26)) return NVMAI_CUDA_ERANGE;
-    if (!aligned_to(idx, 4) || !aligned_to(position, 4) || !aligned_to(source, 4) || !aligned_to(expert_begin, 4)) return NVMAI_CUDA_EINVAL;
-    if ((x == nullptr) != (rows == nullptr)) return NVMAI_CUDA_EINVAL;
-    if (x != nullptr) {
-        if (x_elem > ELEM_BF16 || (rows_elem != x_elem && rows_elem != ELEM_I8)) return NVMAI_CUDA_EINVAL;
-        if (d == 0 || x_stride < d || rows_stride < d) return NVMAI_CUDA_EINVAL;
-        if (!aligned_to(x, elem_size(x_elem)) || !aligned_to(rows, elem_size(rows_elem))) return NVMAI_CUDA_EINVAL;
-        if ((rows_elem == ELEM_I8) != (row_scales != nullptr) || !aligned_to(row_scales, 4)) return NVMAI_CUDA_EINVAL;
-    }
-    const uint64_t counts_bytes = nvmai_cuda_moe_sort_rows_workspace(tokens, top_k, num_experts);
-    if (workspace_bytes < counts_bytes) return NVMAI_CUDA_ERANGE;
-    if (counts_bytes != 0 && (!workspace || !aligned_to(workspace, 16))) return NVMAI_CUDA_EINVAL;
-    if (!on_current_device({idx, position, source, expert_begin, x, rows, row_scales, counts_bytes != 0 ? workspace : nullptr})) return NVMAI_CUDA_EINVAL;
-    const SortParams p{idx, tokens, top_k, num_experts, position, source, expert_begin, x, x_stride, d, rows, rows_stride, row_scales,
-                       counts_bytes != 0 ? static_cast<uint32_t *>(workspace) : nullptr};
-    const dim3 grid(sort_blocks(tokens, top_k)), block(kSortThreads);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.counts != nullptr)
-        if (const int rc = launched(launch_pdl(sort_count_kernel, grid, dim3(512), 0, st, true, p))) return rc;
-    if (x == nullptr) return launched(launch_pdl(sort_rows_kernel<float, 1, 0>, grid, block, 0, st, true, p));
-    return with_pieces(x_elem, d, {{x, x_stride, elem_size(x_elem)}, {rows, rows_stride, elem_size(rows_elem)}}, [&](auto T, auto V) {
-        constexpr int v = decltype(V)::value;
-        if (rows_elem == ELEM_I8) return launched(launch_pdl(sort_rows_kernel<decltype(T), v, 2>, grid, block, 0, st, true, p));
-        return launched(launch_pdl(sort_rows_kernel<decltype(T), v, 1>, grid, block, 0, st, true, p));
+    return without_exceptions([&]() -> int {
+        if (!expert_begin || (tokens != 0 && (!idx || !position || !source))) return NVMAI_CUDA_EINVAL;
+        if (top_k == 0 || top_k > kRowMaxTopK || num_experts == 0 || num_experts > kRowMaxExperts) return NVMAI_CUDA_ERANGE;
+        if ((uint64_t)tokens * top_k >= (1ull << 26)) return NVMAI_CUDA_ERANGE;
+        if (!aligned_to(idx, 4) || !aligned_to(position, 4) || !aligned_to(source, 4) || !aligned_to(expert_begin, 4)) return NVMAI_CUDA_EINVAL;
+        if ((x == nullptr) != (rows == nullptr)) return NVMAI_CUDA_EINVAL;
+        if (x != nullptr) {
+            if (x_elem > ELEM_BF16 || (rows_elem != x_elem && rows_elem != ELEM_I8)) return NVMAI_CUDA_EINVAL;
+            if (d == 0 || x_stride < d || rows_stride < d) return NVMAI_CUDA_EINVAL;
+            if (!aligned_to(x, elem_size(x_elem)) || !aligned_to(rows, elem_size(rows_elem))) return NVMAI_CUDA_EINVAL;
+            if ((rows_elem == ELEM_I8) != (row_scales != nullptr) || !aligned_to(row_scales, 4)) return NVMAI_CUDA_EINVAL;
+        }
+        const uint64_t counts_bytes = nvmai_cuda_moe_sort_rows_workspace(tokens, top_k, num_experts);
+        if (workspace_bytes < counts_bytes) return NVMAI_CUDA_ERANGE;
+        if (counts_bytes != 0 && (!workspace || !aligned_to(workspace, 16))) return NVMAI_CUDA_EINVAL;
+        if (!on_current_device({idx, position, source, expert_begin, x, rows, row_scales, counts_bytes != 0 ? workspace : nullptr})) return NVMAI_CUDA_EINVAL;
+        const SortParams p{idx, tokens, top_k, num_experts, position, source, expert_begin, x, x_stride, d, rows, rows_stride, row_scales,
+                           counts_bytes != 0 ? static_cast<uint32_t *>(workspace) : nullptr};
+        const dim3 grid(sort_blocks(tokens, top_k)), block(kSortThreads);
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (p.counts != nullptr)
+            if (const int rc = launched(launch_pdl(sort_count_kernel, grid, dim3(512), 0, st, true, p))) return rc;
+        if (x == nullptr) return launched(launch_pdl(sort_rows_kernel<float, 1, 0>, grid, block, 0, st, true, p));
+        return with_pieces(x_elem, d, {{x, x_stride, elem_size(x_elem)}, {rows, rows_stride, elem_size(rows_elem)}}, [&](auto T, auto V) {
+            constexpr int v = decltype(V)::value;
+            if (rows_elem == ELEM_I8) return launched(launch_pdl(sort_rows_kernel<decltype(T), v, 2>, grid, block, 0, st, true, p));
+            return launched(launch_pdl(sort_rows_kernel<decltype(T), v, 1>, grid, block, 0, st, true, p));
+    });
     });
 }
 
 int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_t rows_stride, uint32_t n_rows, const uint32_t *position,
                               const void *w, uint32_t w_elem, uint32_t tokens, uint32_t top_k, uint32_t d, const void *base,
                               uint32_t base_stride, void *y, uint32_t y_stride, void *stream) {
-    if ((n_rows != 0 && !rows) || (tokens != 0 && (!position || !y))) return NVMAI_CUDA_EINVAL;
-    if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
-    if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
-    if (d == 0 || y_stride < d || (n_rows != 0 && rows_stride < d) || (base && base_stride < d)) return NVMAI_CUDA_EINVAL;
-    const size_t size = elem_size(elem);
-    if (!aligned_to(rows, size) || !aligned_to(y, size) || !aligned_to(base, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
-        !aligned_to(position, 4))
-        return NVMAI_CUDA_EINVAL;
-    if (tokens == 0) return NVMAI_CUDA_OK;
-    if (!on_current_device({n_rows != 0 ? rows : nullptr, position, w, base, y})) return NVMAI_CUDA_EINVAL;
-    const MergeParams p{rows, rows_stride, n_rows, position, w, w_elem, tokens, top_k, d, base, base_stride, y, y_stride};
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const std::initializer_list<Rows> all{{n_rows != 0 ? rows : nullptr, rows_stride, size}, {base, base_stride, size}, {y, y_stride, size}};
-    auto narrow = [&](auto T) {
-        uint32_t tx = 32;
-        while (tx < 256 && tx * 4 < d) tx *= 2;
-        const uint32_t ty = 256 / tx;
-        return launched(launch_pdl(merge_narrow_kernel<decltype(T)>, dim3((tokens + ty - 1) / ty), dim3(tx, ty), 0, st, true, p));
-    };
-    auto go = [&](auto T, auto V) {
-        using std::integral_constant;
-        constexpr uint32_t piece = sizeof(T) * decltype(V)::value;
-        if constexpr (piece < 4) {
-            return narrow(T);
-        } else {
-            constexpr int r = piece == 16 ? 1 : 4;               // 4-byte pieces: four times as many of them a step
-            const size_t smem = 8 * kMergeAhead * (size_t)merge_stage_bytes(top_k, 32 * r * piece);
-            const uint64_t runs = (uint64_t)tokens * ((d / decltype(V)::value + 32 * r - 1) / (32 * r));
-            const uint64_t resident = kSms * std::min<uint64_t>(8, 220 * 1024 / (smem + 1024));
-            return launched(launch_pdl(merge_rows_kernel<decltype(T), decltype(V)::value, r>, dim3((unsigned)std::min<uint64_t>(resident, (runs + 7) / 8)),
-                                       dim3(256), smem, st, true, p));
-        }
-    };
-    return with_pieces(elem, d, all, go);
+    return without_exceptions([&]() -> int {
+        if ((n_rows != 0 && !rows) || (tokens != 0 && (!position || !y))) return NVMAI_CUDA_EINVAL;
+        if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
+        if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+        if (d == 0 || y_stride < d || (n_rows != 0 && rows_stride < d) || (base && base_stride < d)) return NVMAI_CUDA_EINVAL;
+        const size_t size = elem_size(elem);
+        if (!aligned_to(rows, size) || !aligned_to(y, size) || !aligned_to(base, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
+            !aligned_to(position, 4))
+            return NVMAI_CUDA_EINVAL;
+        if (tokens == 0) return NVMAI_CUDA_OK;
+        if (!on_current_device({n_rows != 0 ? rows : nullptr, position, w, base, y})) return NVMAI_CUDA_EINVAL;
+        const MergeParams p{rows, rows_stride, n_rows, position, w, w_elem, tokens, top_k, d, base, base_stride, y, y_stride};
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const std::initializer_list<Rows> all{{n_rows != 0 ? rows : nullptr, rows_stride, size}, {base, base_stride, size}, {y, y_stride, size}};
+        auto narrow = [&](auto T) {
+            uint32_t tx = 32;
+            while (tx < 256 && tx * 4 < d) tx *= 2;
+            const uint32_t ty = 256 / tx;
+            return launched(launch_pdl(merge_narrow_kernel<decltype(T)>, dim3((tokens + ty - 1) / ty), dim3(tx, ty), 0, st, true, p));
+        };
+        auto go = [&](auto T, auto V) {
+            using std::integral_constant;
+            constexpr uint32_t piece = sizeof(T) * decltype(V)::value;
+            if constexpr (piece < 4) {
+                return narrow(T);
+            } else {
+                constexpr int r = piece == 16 ? 1 : 4;               // 4-byte pieces: four times as many of them a step
+                const size_t smem = 8 * kMergeAhead * (size_t)merge_stage_bytes(top_k, 32 * r * piece);
+                const uint64_t runs = (uint64_t)tokens * ((d / decltype(V)::value + 32 * r - 1) / (32 * r));
+                const uint64_t resident = kSms * std::min<uint64_t>(8, 220 * 1024 / (smem + 1024));
+                return launched(launch_pdl(merge_rows_kernel<decltype(T), decltype(V)::value, r>, dim3((unsigned)std::min<uint64_t>(resident, (runs + 7) / 8)),
+                                           dim3(256), smem, st, true, p));
+            }
+        };
+        return with_pieces(elem, d, all, go);
+    });
 }
 
 int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_stride, const void *rows, uint32_t rows_stride,
                                    uint32_t n_rows, const uint32_t *position, const void *w, uint32_t w_elem, uint32_t tokens,
                                    uint32_t top_k, uint32_t d, void *drows, uint32_t drows_stride, float *dw, void *stream) {
-    if ((!drows && !dw) || (tokens != 0 && (!dy || !position))) return NVMAI_CUDA_EINVAL;
-    if (dw && n_rows != 0 && !rows) return NVMAI_CUDA_EINVAL;
-    if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
-    if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
-    if (d == 0 || dy_stride < d || (drows && drows_stride < d) || (dw && n_rows != 0 && rows_stride < d)) return NVMAI_CUDA_EINVAL;
-    const size_t size = elem_size(elem);
-    if (!aligned_to(dy, size) || !aligned_to(rows, size) || !aligned_to(drows, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
-        !aligned_to(dw, 4) || !aligned_to(position, 4))
-        return NVMAI_CUDA_EINVAL;
-    if (tokens == 0) return NVMAI_CUDA_OK;
-    const void *read = dw && n_rows != 0 ? rows : nullptr;       // the rows are read for dw alone
-    if (!on_current_device({dy, read, position, w, n_rows != 0 ? drows : nullptr, dw})) return NVMAI_CUDA_EINVAL;
-    const uint32_t pairs = tokens * top_k;
-    const MergeGradParams p{dy, dy_stride, rows, rows_stride, n_rows, position, w, w_elem, pairs, top_k, d, drows, drows_stride, dw};
-    return with_pieces(elem, d, {{dy, dy_stride, size}, {read, rows_stride, size}, {drows, drows_stride, size}}, [&](auto T, auto V) {
-        return launched(launch_pdl(merge_rows_grad_kernel<decltype(T), decltype(V)::value>, dim3((pairs + 7) / 8), dim3(256), 0,
-                                   static_cast<cudaStream_t>(stream), true, p));
+    return without_exceptions([&]() -> int {
+        if ((!drows && !dw) || (tokens != 0 && (!dy || !position))) return NVMAI_CUDA_EINVAL;
+        if (dw && n_rows != 0 && !rows) return NVMAI_CUDA_EINVAL;
+        if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
+        if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+        if (d == 0 || dy_stride < d || (drows && drows_stride < d) || (dw && n_rows != 0 && rows_stride < d)) return NVMAI_CUDA_EINVAL;
+        const size_t size = elem_size(elem);
+        if (!aligned_to(dy, size) || !aligned_to(rows, size) || !aligned_to(drows, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
+            !aligned_to(dw, 4) || !aligned_to(position, 4))
+            return NVMAI_CUDA_EINVAL;
+        if (tokens == 0) return NVMAI_CUDA_OK;
+        const void *read = dw && n_rows != 0 ? rows : nullptr;       // the rows are read for dw alone
+        if (!on_current_device({dy, read, position, w, n_rows != 0 ? drows : nullptr, dw})) return NVMAI_CUDA_EINVAL;
+        const uint32_t pairs = tokens * top_k;
+        const MergeGradParams p{dy, dy_stride, rows, rows_stride, n_rows, position, w, w_elem, pairs, top_k, d, drows, drows_stride, dw};
+        return with_pieces(elem, d, {{dy, dy_stride, size}, {read, rows_stride, size}, {drows, drows_stride, size}}, [&](auto T, auto V) {
+            return launched(launch_pdl(merge_rows_grad_kernel<decltype(T), decltype(V)::value>, dim3((pairs + 7) / 8), dim3(256), 0,
+                                       static_cast<cudaStream_t>(stream), true, p));
+    });
     });
 }
 
 int nvmai_cuda_moe_quantize_rows(const void *x, uint32_t elem, uint32_t x_stride, uint32_t rows, uint32_t n, void *q, uint32_t q_stride,
                                  float *scales, void *stream) {
-    if (rows != 0 && (!x || !q || !scales)) return NVMAI_CUDA_EINVAL;
-    if (elem > ELEM_BF16 || n == 0 || x_stride < n || q_stride < n) return NVMAI_CUDA_EINVAL;
-    if (!aligned_to(x, elem_size(elem)) || !aligned_to(scales, 4)) return NVMAI_CUDA_EINVAL;
-    if (rows == 0) return NVMAI_CUDA_OK;
-    if (!on_current_device({x, q, scales})) return NVMAI_CUDA_EINVAL;
-    return launched(launch_quantize(x, elem, x_stride, rows, n, static_cast<int8_t *>(q), q_stride, scales,
-                                    static_cast<cudaStream_t>(stream)));
+    return without_exceptions([&]() -> int {
+        if (rows != 0 && (!x || !q || !scales)) return NVMAI_CUDA_EINVAL;
+        if (elem > ELEM_BF16 || n == 0 || x_stride < n || q_stride < n) return NVMAI_CUDA_EINVAL;
+        if (!aligned_to(x, elem_size(elem)) || !aligned_to(scales, 4)) return NVMAI_CUDA_EINVAL;
+        if (rows == 0) return NVMAI_CUDA_OK;
+        if (!on_current_device({x, q, scales})) return NVMAI_CUDA_EINVAL;
+        return launched(launch_quantize(x, elem, x_stride, rows, n, static_cast<int8_t *>(q), q_stride, scales,
+                                        static_cast<cudaStream_t>(stream)));
+    });
 }
 
 }  // extern "C"

@@ -79,3 +79,8 @@ def int8_matmul(a, b, b_scales, out, rows: int, k: int, n: int, *, a_elem: int =
 def int8_matmul_status(stream=None) -> None:
     """Waits for `stream`; raises NvmaiError(ETIMEOUT) if an `int8_matmul` call gave up a device-side wait."""
     check(_lib.lib().nvmai_cuda_moe_int8_matmul_status(_stream(stream)), "int8_matmul_status")
+
+
+def debug_drop_int8_copy() -> None:
+    """Test hook: the next large `int8_matmul` leaves out one copy, so that its bounded waits run out."""
+    check(_lib.lib().nvmai_cuda_moe_debug_drop_int8_copy(), "debug_drop_int8_copy")

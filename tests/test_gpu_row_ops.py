@@ -488,6 +488,30 @@ def test_product_by_expert(rows, k, n, experts, kind, activation):
     check_product(rows, k, n, activation, out=("fp16", "fp32")[rows % 2], experts=experts, begin=spread(rows + experts, rows, experts, kind))
 
 
+@pytest.mark.parametrize("activation", [fmt.ACT_NONE, fmt.ACT_SILU])
+@pytest.mark.parametrize("k,n", [(512, 136), (2048, 24), (700, 33)])
+def test_a_rows_bits_do_not_depend_on_the_others(k, n, activation):
+    """the kernels for few and for many rows give the same bits: every prefix of the rows has those of all of them"""
+    most = 200
+    gated = activation != fmt.ACT_NONE
+    a, sa = codes(171, most, k)
+    b, sb = codes(172, n * (2 if gated else 1), k)
+    sb = sb * (0.5 / (k ** 0.5 * 74 * 74))
+    for out in TYPES:
+        t, elem = TYPES[out]
+        y = {}
+        for rows in (1, 7, 16, 31, 32, 33, 100, most):
+            y[rows] = torch.empty((rows, n), dtype=t, device="cuda")
+            nv.int8_matmul(a, b, sb, y[rows], rows, k, n, a_scales=sa, a_stride=a.shape[1], b_stride=b.shape[1], activation=activation, out_elem=elem)
+        for rows in y:
+            assert torch.equal(y[rows], y[most][:rows]), rows
+        begin = torch.tensor([0, 3, 3, 60, most], dtype=torch.int32, device="cuda")     # four experts with the same matrix
+        z = torch.empty((most, n), dtype=t, device="cuda")
+        nv.int8_matmul(a, b.repeat(4, 1), sb.repeat(4), z, most, k, n, a_scales=sa, a_stride=a.shape[1], b_stride=b.shape[1], num_experts=4,
+                       expert_begin=begin, activation=activation, out_elem=elem)
+        assert torch.equal(z, y[most])
+
+
 @pytest.mark.parametrize("a_type", TYPES)
 @pytest.mark.parametrize("rows,experts", [(8, 64), (200, 16), (900, 4)])
 def test_product_by_expert_quantises_its_rows(a_type, rows, experts):
@@ -651,8 +675,41 @@ def test_a_captured_block_replays_on_new_rows_and_streams():
         two.check(new)
 
 
-def test_buffers_of_the_host_are_refused():
-    host, dev = torch.zeros(64, dtype=torch.float32), torch.zeros(64, device="cuda")
+def test_a_wait_that_runs_out_is_reported_and_over():
+    """one copy is left out: the call ends, the status says so once, the next call is right"""
+    from nvmai_b200.moe import debug_set_wait_limit
+    from nvmai_b200.row_ops import debug_drop_int8_copy
+    rows, k, n = 300, 640, 130
+    nv.int8_matmul_status()
+    debug_set_wait_limit(2_000_000)
+    try:
+        for activation in (fmt.ACT_NONE, fmt.ACT_SILU):
+            debug_drop_int8_copy()
+            with pytest.raises(NvmaiError) as ei:
+                check_product(rows, k, n, activation)
+            assert ei.value.code == _lib.ETIMEOUT
+            check_product(rows, k, n, activation)
+    finally:
+        debug_set_wait_limit(0)
+
+
+def test_status_refuses_a_capture():
+    stream = torch.cuda.Stream()
+    x, q, s = torch.zeros(1, 64, device="cuda"), torch.zeros(64, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        nv.quantize_rows(x, 1, 64, q, s, elem=fmt.ELEM_F32, stream=stream)
+        with pytest.raises(NvmaiError) as ei:
+            nv.int8_matmul_status(stream)
+        assert ei.value.code == _lib.EINVAL
+    graph.replay()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("pinned", [False, True])
+def test_buffers_of_the_host_are_refused(pinned):
+    host, dev = torch.zeros(64, dtype=torch.float32, pin_memory=pinned), torch.zeros(64, device="cuda")
     q = torch.zeros(64, dtype=torch.int8, device="cuda")
     for call in (lambda: nv.quantize_rows(host, 1, 64, q, dev, elem=fmt.ELEM_F32),
                  lambda: nv.merge_rows(dev, 1, host, 1, 1, 64, dev, elem=fmt.ELEM_F32),
