@@ -168,22 +168,29 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
             for (uint32_t k = lane; k < p.top_k; k += 32u)
                 if (place[k] != kNoRow) p.row_scales[place[k]] = scale;
         };
-        // a warp takes a token's row, or a part of it where the block has fewer tokens than warps
-        const uint32_t mine = last - first;
-        const uint32_t parts = mine == 0 || mine >= kSortWarps ? 1u : kSortWarps / mine;
-        const uint32_t pieces = p.d / V, each = (pieces + parts - 1u) / parts;
+        // a warp takes a token's row, or a part of it (a piece a lane at least) where the block has fewer tokens than warps
+        const uint32_t mine = last - first, pieces = p.d / V;
+        const uint32_t parts = mine == 0 || mine >= kSortWarps ? 1u : min(kSortWarps / mine, (pieces + 31u) / 32u);
+        const uint32_t each = (pieces + parts - 1u) / parts;
         for (uint32_t u = warp; u < mine * parts; u += kSortWarps) {
             const uint32_t t = first + u / parts, part = u % parts;
             const uint32_t c0 = part * each, c1 = min(pieces, c0 + each);
             const P *src = reinterpret_cast<const P *>(static_cast<const T *>(p.x) + (size_t)t * p.x_stride);
             const uint32_t *place = own + (t - first) * p.top_k;
             if constexpr (MOVE == 1) {
-#pragma unroll 4
-                for (uint32_t c = c0 + lane; c < c1; c += 32u) {
-                    const P v = src[c];
+                // four pieces are requested before any is stored
+                for (uint32_t c = c0 + lane; c < c1; c += 128u) {
+                    P v[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; ++i)
+                        if (c + 32u * i < c1) v[i] = src[c + 32u * i];
                     for (uint32_t k = 0; k < p.top_k; ++k) {
                         const uint32_t row = place[k];
-                        if (row != kNoRow) reinterpret_cast<P *>(static_cast<T *>(p.rows) + (size_t)row * p.rows_stride)[c] = v;
+                        if (row == kNoRow) continue;
+                        P *dst = reinterpret_cast<P *>(static_cast<T *>(p.rows) + (size_t)row * p.rows_stride) + c;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; ++i)
+                            if (c + 32u * i < c1) dst[32u * i] = v[i];
                     }
                 }
             } else {
@@ -196,12 +203,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
                 }
                 m = __reduce_max_sync(0xffffffffu, m);
                 const RowScale rs = row_scale_bits(m);
-#pragma unroll 4
-                for (uint32_t c = c0 + lane; c < c1; c += 32u) {
-                    const Q q = code(src[c], rs);
+                for (uint32_t c = c0 + lane; c < c1; c += 128u) {
+                    Q q[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; ++i)
+                        if (c + 32u * i < c1) q[i] = code(src[c + 32u * i], rs);
                     for (uint32_t k = 0; k < p.top_k; ++k) {
                         const uint32_t row = place[k];
-                        if (row != kNoRow) reinterpret_cast<Q *>(static_cast<int8_t *>(p.rows) + (size_t)row * p.rows_stride)[c] = q;
+                        if (row == kNoRow) continue;
+                        Q *dst = reinterpret_cast<Q *>(static_cast<int8_t *>(p.rows) + (size_t)row * p.rows_stride) + c;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; ++i)
+                            if (c + 32u * i < c1) dst[32u * i] = q[i];
                     }
                 }
                 if (part == 0) scale_out(place, rs.scale);
@@ -391,7 +404,7 @@ struct MergeGradParams {
 
 // A warp per pair; the eight warps of a block share the rows of dy in the L1.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) merge_rows_grad_kernel(MergeGradParams p) {
+__global__ void __launch_bounds__(256, 4) merge_rows_grad_kernel(MergeGradParams p) {
     using P = Piece<T, V>;
     pdl_wait();
     pdl_launch_dependents();
@@ -406,22 +419,32 @@ __global__ void __launch_bounds__(256) merge_rows_grad_kernel(MergeGradParams p)
     const P *dy = reinterpret_cast<const P *>(static_cast<const T *>(p.dy) + (size_t)(pair / p.top_k) * p.dy_stride);
     const P *v = reinterpret_cast<const P *>(static_cast<const T *>(p.rows) + (size_t)row * p.rows_stride);
     P *o = reinterpret_cast<P *>(static_cast<T *>(p.drows) + (size_t)row * p.drows_stride);
+    // kAhead pieces of both rows are requested before any is stored: drows may be rows, so the compiler keeps loads behind stores
+    constexpr int kAhead = V == 8 ? 2 : V == 4 ? 4 : 8;
+    const uint32_t pieces = p.d / V;
     float dot = 0.0f;
-    constexpr int kUnroll = sizeof(P) == 16 ? 4 : 8;
-#pragma unroll kUnroll
-    for (uint32_t c = lane; c < p.d / V; c += 32u) {
-        const P g = dy[c];
-        if (p.dw != nullptr) {
-            const P r = v[c];
+    for (uint32_t c0 = lane; c0 < pieces; c0 += 32u * kAhead) {
+        P gv[kAhead], rv[kAhead];
 #pragma unroll
-            for (int i = 0; i < V; ++i) dot = fmaf(elem_to_float(g.v[i]), elem_to_float(r.v[i]), dot);
-        }
-        if (p.drows != nullptr) {
-            P s;
+        for (int u = 0; u < kAhead; ++u)
+            if (c0 + 32u * u < pieces) {
+                gv[u] = dy[c0 + 32u * u];
+                if (p.dw != nullptr) rv[u] = v[c0 + 32u * u];
+            }
 #pragma unroll
-            for (int i = 0; i < V; ++i) s.v[i] = elem_from_float<T>(w * elem_to_float(g.v[i]));
-            o[c] = s;
-        }
+        for (int u = 0; u < kAhead; ++u)
+            if (c0 + 32u * u < pieces) {
+                if (p.dw != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) dot = fmaf(elem_to_float(gv[u].v[i]), elem_to_float(rv[u].v[i]), dot);
+                }
+                if (p.drows != nullptr) {
+                    P s;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s.v[i] = elem_from_float<T>(w * elem_to_float(gv[u].v[i]));
+                    o[c0 + 32u * u] = s;
+                }
+            }
     }
     if (p.dw != nullptr) {
 #pragma unroll
