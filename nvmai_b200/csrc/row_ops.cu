@@ -274,17 +274,24 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
         const uint32_t k = x.g * kMergeSlots + lane;
         return x.t < p.tokens && lane < kMergeSlots && k < p.top_k ? p.position[(size_t)x.t * p.top_k + k] : kNoRow;
     };
+    // Held slots of a step.  All eight of a whole run, the common case, go without a question for each piece; else only those
+    // that are held are gone through.
+    constexpr uint32_t kAll = (1u << kMergeSlots) - 1u;
+    auto held = [&](uint32_t pos) { return __ballot_sync(0xffffffffu, pos < p.n_rows); };
+    auto whole = [&](const At &x, uint32_t mask) { return mask == kAll && (x.run + 1u) * kRun <= pieces; };
     auto request = [&](const At &x, uint32_t pos, uint32_t slot) {
-        const uint32_t c = x.run * kRun + lane, to = ring_at + slot * stage_bytes;
+        const uint32_t c = x.run * kRun + lane, to = ring_at + slot * stage_bytes, mask = held(pos);
+        auto row = [&](uint32_t k, auto all) {
+            const P *src = reinterpret_cast<const P *>(rows + (size_t)__shfl_sync(0xffffffffu, pos, k) * p.rows_stride) + c;
 #pragma unroll
-        for (uint32_t k = 0; k < kMergeSlots; ++k) {
-            const uint32_t row = __shfl_sync(0xffffffffu, pos, k);
-            if (row < p.n_rows) {
-                const P *src = reinterpret_cast<const P *>(rows + (size_t)row * p.rows_stride) + c;
+            for (uint32_t r = 0; r < R; ++r)
+                if (decltype(all)::value || c + r * 32u < pieces) cp_async(to + k * kRunBytes + r * 32u * kPiece, src + r * 32u, kPiece);
+        };
+        if (whole(x, mask)) {
 #pragma unroll
-                for (uint32_t r = 0; r < R; ++r)
-                    if (c + r * 32u < pieces) cp_async(to + k * kRunBytes + r * 32u * kPiece, src + r * 32u, kPiece);
-            }
+            for (uint32_t k = 0; k < kMergeSlots; ++k) row(k, std::true_type{});
+        } else {
+            for (uint32_t m = mask; m != 0u; m &= m - 1u) row(__ffs((int)m) - 1u, std::false_type{});
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -313,19 +320,22 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
         const bool weighs = p.w != nullptr && lane < kMergeSlots && now_pos < p.n_rows;
         const float mine = weighs ? load_elem(p.w, p.w_elem, (size_t)now.t * p.top_k + now.g * kMergeSlots + lane) : 1.0f;
         asm volatile("cp.async.wait_group %0;" ::"n"(kMergeAhead - 1) : "memory");
-#pragma unroll
-        for (uint32_t k = 0; k < kMergeSlots; ++k) {
-            const uint32_t row = __shfl_sync(0xffffffffu, now_pos, k);
+        auto add = [&](uint32_t k, auto all) {
             const float w = __shfl_sync(0xffffffffu, mine, k);
-            if (row < p.n_rows) {
 #pragma unroll
-                for (uint32_t r = 0; r < R; ++r) {
-                    if (c + r * 32u >= pieces) continue;
-                    const P v = *reinterpret_cast<const P *>(ring + slot * stage_bytes + k * kRunBytes + r * 32u * kPiece);
+            for (uint32_t r = 0; r < R; ++r) {
+                if (!decltype(all)::value && c + r * 32u >= pieces) continue;
+                const P v = *reinterpret_cast<const P *>(ring + slot * stage_bytes + k * kRunBytes + r * 32u * kPiece);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) acc[r][i] = fmaf(w, elem_to_float(v.v[i]), acc[r][i]);
-                }
+                for (int i = 0; i < V; ++i) acc[r][i] = fmaf(w, elem_to_float(v.v[i]), acc[r][i]);
             }
+        };
+        const uint32_t mask = held(now_pos);
+        if (whole(now, mask)) {
+#pragma unroll
+            for (uint32_t k = 0; k < kMergeSlots; ++k) add(k, std::true_type{});
+        } else {
+            for (uint32_t m = mask; m != 0u; m &= m - 1u) add(__ffs((int)m) - 1u, std::false_type{});
         }
         if (now.g + 1u == groups) {
 #pragma unroll
