@@ -71,9 +71,9 @@ struct IgTile { uint32_t subs, nt; };
 
 // Rows of a unit where the rows are spread over experts.  An expert's codes come once for each of its units (past the first from
 // the L2), so a unit holds the average expert and 2.5 times the spread of an even routing around it.  Past 128 rows
-// that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 115.5 us, 160 111.2,
-// 192 118.4 (three ring slots instead of four); 512 -> 2048: 75.7, 68.1, 71.1.  Two channel tiles a unit read the rows half
-// as often: 201 tokens down 50.6 us with one, 46.9 with two.
+// that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 118.0 us, 160 110.5,
+// 192 113.7 (three ring slots instead of four); 512 -> 2048: 72.6, 69.7, 67.7.  Two channel tiles a unit read the rows half
+// as often: 201 tokens, 512 -> 2048, 54.1 us with one, 46.7 with two.
 IgTile grouped_tile(const Matmul &m) {
     const float average = (float)m.rows / (float)m.E;
     const uint32_t want = (uint32_t)std::ceil((average + 2.5f * std::sqrt(average)) / 32.0f) * 32u;
@@ -83,7 +83,7 @@ IgTile grouped_tile(const Matmul &m) {
 // One matrix: the cheapest tile by a model of the time, in ns, fitted to 16 shapes (40 to 16384 rows, 512 to 2048 codes, 300 to 2048
 // channels): a K block costs 104 and 4.1 for each KB of it, the last epilogue of a block 10 for each row and tile of its unit (an
 // activation counts double), earlier ones 6.5 beside the next unit or, with one set of accumulators, 10 in its way.  The
-// tile it picks took at most 7 % longer than the best one in those shapes; always 2 x 128 took up to 45 % longer.
+// tile it picks took at most 9 % longer than the best one in those shapes, 128 rows of two tiles up to 80 %.
 IgTile dense_tile(const Matmul &m) {
     const bool gated = m.act != kActNone;
     const float blocks = (float)((m.k + 127) / 128);
@@ -134,17 +134,19 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     return m.out_elem == ELEM_F16 ? go(__half{}) : m.out_elem == ELEM_BF16 ? go(__nv_bfloat16{}) : go(float{});
 }
 
-// The streaming kernel's tiles of 8 rows, 0: the tcgen05 kernel's.  One matrix: up to 32 rows (codes, 2048 -> 2 x 512 on a B200: 1 row
-// 3.2 us against 7.3, 16 rows 4.2 / 7.3, 32 rows 5.9 / 7.4).  By expert a block has the rows of one, and every one fetches
-// its codes anew: while rows x k is below 2^15 (8 rows of 2048: 6.4 / 10.0 us, 16 rows 11.3 / 11.6, 24 rows 15.7 / 14.0; 32 rows of 512
-// 10.1 / 10.5, 64 rows 16.4 / 14.9).
+// The streaming kernel's tiles of 8 rows, 0: the tcgen05 kernel's.  One matrix: up to 16 rows, up to 32 where the tcgen05 kernel would
+// go through eight K blocks or more one after the other (codes on a B200, streaming / tcgen05: 2048 -> 2 x 512, 1 row 3.1 / 7.6 us,
+// 16 rows 4.1 / 7.6, 32 rows 5.9 / 7.7; 512 -> 2048, 16 rows 3.1 / 3.9, 32 rows 4.3 / 4.0; 1024 -> 1024, 32 rows 4.2 / 4.7).  By
+// expert a block has the rows of one, and every one fetches its codes anew: while rows x k is below 2^15 (8 rows of 2048: 6.7 /
+// 10.7 us, 16 rows 11.7 / 12.1, 24 rows 16.2 / 14.4; 32 rows of 512 10.5 / 10.5, 64 rows 17.3 / 15.0).
 uint32_t stream_tiles(const Matmul &m) {
-    if (m.begin != nullptr ? (uint64_t)m.rows * m.k >= 32768 || m.rows > 64 : m.rows > 32) return 0;
+    if (m.begin != nullptr ? (uint64_t)m.rows * m.k >= 32768 || m.rows > 64 : m.rows > (m.k >= 1024 ? 32u : 16u)) return 0;
     const uint32_t nt = m.begin != nullptr || m.rows <= 8 ? 1 : m.rows <= 16 ? 2 : 4;
     return is_smem(m.k, nt) <= 200 * 1024 ? nt : 0;
 }
-// Does it quantise the rows itself?  Each of its blocks then does, 0.6 us a row in front of the product; a launch for all of
-// them runs beside the fetching of the codes (2048 -> 2 x 512: 1 row 3.9 us in one launch, 4 rows 5.6, in two launches 4.6).
+// Does it quantise the rows itself?  Each of its blocks then does, 0.5 us a row in front of the product; a launch for all of
+// them runs beside the fetching of the codes, and costs the host 2.4 us (2048 -> 2 x 512, one launch / two: 1 row 3.8 / 4.3 us, 2
+// rows 4.5 / 4.1, 4 rows 5.6 / 4.1; one token through eight experts 7.9 / 7.4).
 bool stream_quantizes(const Matmul &m) { return m.begin != nullptr || m.rows <= 2; }
 
 cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
@@ -154,7 +156,8 @@ cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
                m.out, m.out_elem, m.out_stride, m.ready, is_row_bytes(m.k), 1};
     const uint32_t steps = (m.k + kIsStep - 1) / kIsStep, columns = m.begin != nullptr ? m.rows : (m.rows + 8 * nt - 1) / (8 * nt);
     auto blocks = [&] { return (m.n * p.parts + (gated ? 8 : 16) * kIsWarps - 1) / ((gated ? 8 : 16) * kIsWarps); };    // across the features
-    while (p.parts < kIsWarps && p.parts < steps && (steps > p.parts * kIsAhead || (uint64_t)blocks() * columns < kSms)) p.parts *= 2;
+    const uint64_t resident = nt == 1 ? 2 * kSms : kSms;                 // blocks
+    while (p.parts < kIsWarps && p.parts < steps && (steps > p.parts * kIsAhead || 2 * (uint64_t)blocks() * columns <= resident)) p.parts *= 2;
     const dim3 grid(blocks(), columns);
     auto go = [&](auto T, auto V, auto G, auto N) {
         return launch_pdl(int8_stream_kernel<decltype(T), decltype(V)::value, decltype(G)::value, decltype(N)::value>, grid,

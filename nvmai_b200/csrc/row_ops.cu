@@ -240,8 +240,8 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int byte
 // A warp sums a run of 32 R pieces of V neighbouring elements of a token and goes on to the next run, as many warps further as
 // there are.  A step is a run's pieces of up to eight slots; a step is copied into shared memory while the one before is
 // added, each lane its own pieces, so that a lane waits for its own copies alone (cp.async groups) and no registers hold what is
-// in flight: 24 warps an SM with a step of 4 KB each.  4096 tokens of eight 4 KB rows on a B200: 26.6 us, 5.7 TB/s; a thread per piece
-// without the ring 35.2 (the rows' latency is exposed), a ring of four steps 56 (12 warps an SM, too few for the instructions).
+// in flight: 24 warps an SM with a step of 4 KB each.  4096 tokens of eight 4 KB rows on a B200: 25.4 us, 5.9 TB/s; a thread per piece
+// without the ring 35.2 (the rows' latency is exposed), a ring of four steps 56 (8 warps an SM, too few for the instructions).
 constexpr uint32_t kMergeSlots = 8, kMergeAhead = 2;
 __host__ __device__ constexpr uint32_t merge_stage_bytes(uint32_t top_k, uint32_t run_bytes) {
     return (top_k < kMergeSlots ? top_k : kMergeSlots) * run_bytes;
@@ -354,10 +354,10 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
     }
 }
 
-// Rows of 16-bit elements that share no 4-byte boundary: a thread sums every 32nd element, four of them and two slots at a time.
+// Rows of 16-bit elements that share no 4-byte boundary: a thread sums every 32nd element, four of them and four slots at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) merge_narrow_kernel(MergeParams p) {
-    constexpr int U = 4, kAhead = 2;
+    constexpr int U = 4, kAhead = 4;
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t t = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31u;
@@ -471,8 +471,7 @@ struct QuantizeParams {
 };
 
 // WARPS warps per row, which they hold in registers between the largest magnitude and the codes; a longer row is read twice.
-// 4096 rows of 2048 fp16 elements on a B200: see the table of the documents for times; one row of 2048 takes eight warps 1.9 us,
-// one warp 2.6.
+// Reading bounds it: 4096 rows of 2048 fp16 elements 5.2 us on a B200, 4.8 TB/s.
 constexpr int kQuantizeHeld = 8;             // pieces of a row that a lane holds
 template <typename T, int V, int WARPS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p) {
@@ -560,8 +559,9 @@ cudaError_t nvmai::launch_quantize(const void *x, uint32_t elem, uint32_t x_stri
     const QuantizeParams p{x, x_stride, rows, n, q, q_stride, scales};
     return with_pieces(elem, n, {{x, x_stride, elem_size(elem)}, {q, q_stride, 1}}, [&](auto T, auto V) {
         constexpr int v = decltype(V)::value;
-        // A block per row where a warp each would leave SMs with less than eight, or could not hold its row
-        if (rows < 8 * kSms || n > 32u * kQuantizeHeld * v)
+        // Eight warps a row for few rows, and for rows that one warp cannot hold (fp16, one warp / eight: 1 x 2048 2.0 / 1.6 us,
+        // 201 x 2048 2.5 / 2.0, 1000 x 2048 2.6 / 3.6, 32768 x 512 12.8 / 67.7, 300 x 8000 13.1 / 3.4)
+        if (rows < 3 * kSms || n > 32u * kQuantizeHeld * v)
             return launch_pdl(quantize_rows_kernel<decltype(T), v, 8>, dim3(rows), dim3(256), 0, st, true, p);
         return launch_pdl(quantize_rows_kernel<decltype(T), v, 1>, dim3((rows + 7) / 8), dim3(256), 0, st, true, p);
     });
