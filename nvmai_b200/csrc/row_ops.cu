@@ -100,11 +100,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(SortParams p) {
     pdl_launch_dependents();
     for (uint32_t i = lo + tid; i < hi; i += kSortThreads) own[i - lo] = min(p.idx[i], p.E);
     if (p.counts == nullptr) {
+        auto count = [&](uint32_t i, uint32_t e) { atomicAdd(i < lo ? &before[min(e, p.E)] : &rest[min(e, p.E)], 1u); };
+        const uint32_t fours = (reinterpret_cast<uintptr_t>(p.idx) & 15u) == 0u ? pairs / 4u : 0u;
 #pragma unroll 4
-        for (uint32_t i = tid; i < pairs; i += kSortThreads) {
-            const uint32_t e = min(p.idx[i], p.E);
-            atomicAdd(i < lo ? &before[e] : &rest[e], 1u);
+        for (uint32_t i = tid; i < fours; i += kSortThreads) {
+            const uint4 e = reinterpret_cast<const uint4 *>(p.idx)[i];
+            count(4u * i, e.x); count(4u * i + 1u, e.y); count(4u * i + 2u, e.z); count(4u * i + 3u, e.w);
         }
+        for (uint32_t i = 4u * fours + tid; i < pairs; i += kSortThreads) count(i, p.idx[i]);
     } else {
         // 128 neighbouring experts a warp, the blocks spread over the warps that share them
         const uint32_t columns = sort_columns(p.E), across = (columns + 127u) / 128u, shares = kSortWarps / across;
