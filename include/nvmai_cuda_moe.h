@@ -457,7 +457,7 @@ NVMAI_API int nvmai_cuda_moe_residual_add_f16(void *hidden, const void *delta, u
  * one row to the next and are at least the row's length.  All pointers are memory of the current
  * device, or managed memory (NVMAI_CUDA_EINVAL otherwise); indexes and positions are checked on
  * the device, an entry out of range counts as not held, never as an address.  Outputs overlap
- * neither inputs nor each other, except where a call says so. */
+ * neither inputs nor each other, except where a call says so.  Rows have at most 2^30 elements. */
 
 /* Sorts the tokens * top_k pairs (token t, slot k), pair = t * top_k + k, by expert: pairs with
  * idx[pair] < num_experts are kept, ordered by (expert, pair); the others (a padded row's, another
@@ -489,7 +489,8 @@ NVMAI_API int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_
 
 /* Gradients of merge_rows: drows[position[t][k]] = w[t][k] * dy[t] (rounded to `elem`; rows that no
  * position names are left as they were) and dw[t][k] = sum over i of dy[t][i] * rows[position[t][k]][i]
- * (fp32; 0 where the position is not held).  w = NULL: weights of 1.  Either of drows and dw may be NULL;
+ * (fp32; 0 where the position is not held).  Positions are distinct, as sort_rows writes them (a row
+ * that two pairs name gets the product of one of them).  w = NULL: weights of 1.  Either of drows and dw may be NULL;
  * rows may be NULL without dw; drows may be rows itself.  The gradient of base is dy. */
 NVMAI_API int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_stride, const void *rows,
                                              uint32_t rows_stride, uint32_t n_rows, const uint32_t *position,

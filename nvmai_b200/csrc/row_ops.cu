@@ -596,6 +596,7 @@ int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_
         if (x != nullptr) {
             if (x_elem > ELEM_BF16 || (rows_elem != x_elem && rows_elem != ELEM_I8)) return NVMAI_CUDA_EINVAL;
             if (d == 0 || x_stride < d || rows_stride < d) return NVMAI_CUDA_EINVAL;
+            if (d > kRowMaxLength) return NVMAI_CUDA_ERANGE;
             if (!aligned_to(x, elem_size(x_elem)) || !aligned_to(rows, elem_size(rows_elem))) return NVMAI_CUDA_EINVAL;
             if ((rows_elem == ELEM_I8) != (row_scales != nullptr) || !aligned_to(row_scales, 4)) return NVMAI_CUDA_EINVAL;
         }
@@ -624,7 +625,7 @@ int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_t rows_str
     return without_exceptions([&]() -> int {
         if ((n_rows != 0 && !rows) || (tokens != 0 && (!position || !y))) return NVMAI_CUDA_EINVAL;
         if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
-        if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+        if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31) || d > kRowMaxLength) return NVMAI_CUDA_ERANGE;
         if (d == 0 || y_stride < d || (n_rows != 0 && rows_stride < d) || (base && base_stride < d)) return NVMAI_CUDA_EINVAL;
         const size_t size = elem_size(elem);
         if (!aligned_to(rows, size) || !aligned_to(y, size) || !aligned_to(base, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
@@ -666,7 +667,7 @@ int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_st
         if ((!drows && !dw) || (tokens != 0 && (!dy || !position))) return NVMAI_CUDA_EINVAL;
         if (dw && n_rows != 0 && !rows) return NVMAI_CUDA_EINVAL;
         if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
-        if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31)) return NVMAI_CUDA_ERANGE;
+        if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31) || d > kRowMaxLength) return NVMAI_CUDA_ERANGE;
         if (d == 0 || dy_stride < d || (drows && drows_stride < d) || (dw && n_rows != 0 && rows_stride < d)) return NVMAI_CUDA_EINVAL;
         const size_t size = elem_size(elem);
         if (!aligned_to(dy, size) || !aligned_to(rows, size) || !aligned_to(drows, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
@@ -689,6 +690,7 @@ int nvmai_cuda_moe_quantize_rows(const void *x, uint32_t elem, uint32_t x_stride
     return without_exceptions([&]() -> int {
         if (rows != 0 && (!x || !q || !scales)) return NVMAI_CUDA_EINVAL;
         if (elem > ELEM_BF16 || n == 0 || x_stride < n || q_stride < n) return NVMAI_CUDA_EINVAL;
+        if (n > kRowMaxLength) return NVMAI_CUDA_ERANGE;
         if (!aligned_to(x, elem_size(elem)) || !aligned_to(scales, 4)) return NVMAI_CUDA_EINVAL;
         if (rows == 0) return NVMAI_CUDA_OK;
         if (!on_current_device({x, q, scales})) return NVMAI_CUDA_EINVAL;

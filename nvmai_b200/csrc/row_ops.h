@@ -9,6 +9,7 @@ namespace nvmai {
 
 enum : uint32_t { ELEM_F16 = 0, ELEM_F32 = 1, ELEM_BF16 = 2, ELEM_I8 = 3 };
 constexpr uint32_t kRowMaxExperts = 1024, kRowMaxTopK = 64;
+constexpr uint32_t kRowMaxLength = 1u << 30;       // elements of a row: counts of pieces and their steps stay in 32 bits
 
 inline size_t elem_size(uint32_t e) { return e == ELEM_F32 ? 4 : e == ELEM_I8 ? 1 : 2; }
 inline bool aligned_to(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -153,6 +153,7 @@ def test_no_tokens_leaves_empty_experts():
 ROWS = [  # tokens, top_k, experts, d, x_pad, rows_pad, offset, drop
     (1, 8, 256, 2048, 0, 0, 0, 0.0), (5, 3, 4, 1, 0, 0, 0, 0.4), (7, 2, 9, 37, 0, 0, 1, 0.0), (33, 8, 16, 64, 8, 16, 8, 0.3),
     (150, 8, 256, 2048, 0, 0, 0, 0.5), (201, 5, 100, 999, 3, 2, 0, 0.1), (300, 1, 8, 520, 0, 8, 0, 0.0),
+    (9001, 8, 64, 40, 0, 0, 0, 0.2), (6000, 3, 200, 33, 0, 0, 0, 0.0),
 ]
 
 
@@ -311,6 +312,69 @@ def test_positions_out_of_range_are_never_addresses():
     assert torch.equal(y, torch.stack([rows[0], rows[4], rows[1], torch.zeros(d, device="cuda")]))
     assert torch.equal(drows[[0, 4, 1]], dy[:3]) and (drows[2:4] == 77).all()
     assert dw[0, 1] == 0 and dw[1, 1] == 0 and dw[2, 0] == 0 and (dw[3] == 0).all()
+
+
+def test_a_row_named_twice():
+    """forward every naming counts; the gradient's row is the product of one of the two"""
+    tokens, k, d = 3, 2, 40
+    pos = torch.tensor([[0, 0], [1, 0], [2, 1]], dtype=torch.int32, device="cuda")
+    rows, dy = randn(45, 3, d), randn(46, tokens, d)
+    y, drows, dw = torch.empty(tokens, d, device="cuda"), torch.empty(3, d, device="cuda"), torch.empty(tokens, k, device="cuda")
+    nv.merge_rows(rows, 3, pos, tokens, k, d, y, elem=fmt.ELEM_F32)
+    assert torch.equal(y, torch.stack([rows[0] + rows[0], rows[1] + rows[0], rows[2] + rows[1]]))
+    nv.merge_rows_grad(dy, rows, 3, pos, None, tokens, k, d, drows, dw, elem=fmt.ELEM_F32)
+    for r, names in enumerate(([0, 1], [1, 2], [2])):
+        assert all(any(v == dy[t, i] for t in names) for i, v in enumerate(drows[r]))
+    terms = rows[pos.long()].double() * dy.double()[:, None]
+    assert ((dw.double() - terms.sum(2)).abs() <= d * U * terms.abs().sum(2) * 1.01).all()
+
+
+@pytest.mark.parametrize("d", [64, 63])
+def test_rows_between_kernels_of_other_streams(d):
+    """two calls at once on two streams, each with buffers of its own, while the default stream is busy"""
+    tokens, k, e = 257, 4, 16
+    jobs = []
+    for i in range(2):
+        idx = random_idx(tokens, k, e, 300 + i, 0.1)
+        x = randn(302 + i, tokens, d).half()
+        bufs = dict(position=torch.empty_like(idx), source=torch.empty(tokens * k, dtype=torch.int32, device="cuda"),
+                    begin=torch.empty(e + 1, dtype=torch.int32, device="cuda"), rows=torch.zeros(tokens * k, d, dtype=torch.float16, device="cuda"),
+                    y=torch.empty(tokens, d, dtype=torch.float16, device="cuda"))
+        jobs.append((idx, x, bufs, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    busy = torch.randn(4096, 4096, device="cuda")
+    for _ in range(20):
+        busy = busy @ busy * 1e-3
+        for idx, x, b, stream in jobs:
+            nv.sort_rows(idx, tokens, k, e, b["position"], b["source"], b["begin"], x=x, d=d, rows=b["rows"], stream=stream)
+            nv.merge_rows(b["rows"], tokens * k, b["position"], tokens, k, d, b["y"], stream=stream)
+    torch.cuda.synchronize()
+    for idx, x, b, _ in jobs:
+        check_order(idx, e, b["position"], b["source"], b["begin"])
+        held = (b["position"] >= 0).double().sum(1, keepdim=True)
+        want = x.double() * held                       # the same row, as many times as it is held: exact in fp32, rounded once
+        assert torch.equal(b["y"], want.half())
+
+
+def test_rows_from_a_pointer_inside_a_buffer():
+    """pieces of every width: the same rows from bases 16-, 4- and 2-byte aligned give the same bits"""
+    tokens, k, e, d = 37, 3, 8, 120
+    idx = random_idx(tokens, k, e, 310)
+    x, w = randn(311, tokens, d).bfloat16(), randn(312, tokens, k)
+    outs = []
+    for offset in (0, 2, 1):
+        position, _, begin, rows, _ = sort(idx, e, x, fmt.ELEM_BF16, offset=offset)
+        flat, view = strided(rows, 0, offset)
+        y = torch.empty(offset + tokens * d, dtype=torch.bfloat16, device="cuda")
+        nv.merge_rows(flat, tokens * k, position, tokens, k, d, y[offset:], elem=fmt.ELEM_BF16, w=w, w_elem=fmt.ELEM_F32)
+        q, s = torch.empty(tokens, d, dtype=torch.int8, device="cuda"), torch.empty(tokens, device="cuda")
+        nv.quantize_rows(strided(x, 0, offset)[0], tokens, d, q, s, elem=fmt.ELEM_BF16)
+        dr, dw = torch.empty(offset + tokens * k * d, dtype=torch.bfloat16, device="cuda"), torch.empty(tokens, k, device="cuda")
+        nv.merge_rows_grad(strided(x, 0, offset)[0], flat, tokens * k, position, w, tokens, k, d, dr[offset:], dw, elem=fmt.ELEM_BF16,
+                           w_elem=fmt.ELEM_F32)
+        outs.append((rows, y[offset:].clone(), q, s, dr[offset:].clone()))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
 
 
 # ---- 8-bit codes ---------------------------------------------------------------------------------------------

@@ -53,6 +53,10 @@ E, R = _lib.EINVAL, _lib.ERANGE
     ("sort_rows", SORT, dict(rows_elem=fmt.ELEM_F32), E),
     ("sort_rows", SORT, dict(rows_elem=fmt.ELEM_I8), E),                      # codes without their scales
     ("sort_rows", SORT, dict(row_scales=A), E),                               # scales without codes
+    ("sort_rows", SORT, dict(d=(1 << 30) + 8, x_stride=1 << 31, rows_stride=1 << 31), R),
+    ("merge_rows", MERGE, dict(d=(1 << 30) + 8, rows_stride=1 << 31, base_stride=1 << 31, y_stride=1 << 31), R),
+    ("merge_rows_grad", GRAD, dict(d=(1 << 30) + 8, dy_stride=1 << 31, rows_stride=1 << 31, drows_stride=1 << 31), R),
+    ("quantize_rows", QUANT, dict(n=(1 << 30) + 8, x_stride=1 << 31, q_stride=1 << 31), R),
     ("merge_rows", MERGE, dict(rows=None), E),
     ("merge_rows", MERGE, dict(position=None), E),
     ("merge_rows", MERGE, dict(y=None), E),
