@@ -25,6 +25,7 @@ struct IgParams {
     uint32_t act;
     void *out; size_t out_stride;
     uint32_t nt, stages;                 // most rows of a unit (a multiple of 32), ring slots
+    uint32_t evict_first;                // the matrix's lines leave the L2 before others
     uint32_t accs;                       // sets of accumulators (2, or 1 where two do not fit)
     uint32_t ready;                      // the kernel in front made the rows' codes and nothing else that is read here
     uint32_t paired;                     // 16-bit outputs: two neighbouring channels go out in one store
@@ -79,6 +80,18 @@ __device__ __forceinline__ float gate_act(float g, uint32_t act) {
         return g * r;
     }
     return hidden_act(g, act);
+}
+
+// A box of the matrix whose lines are the first to leave the L2.
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t v;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(v));
+    return v;
+}
+__device__ __forceinline__ void tma_load_2d_once(uint32_t dst_smem, const CUtensorMap *map, uint32_t c0, uint32_t c1, uint64_t *bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;"
+                 ::"r"(dst_smem), "l"(map), "r"(c0), "r"(c1), "r"(smem_addr(bar)), "l"(policy)
+                 : "memory");
 }
 
 struct IgShared {
@@ -197,13 +210,18 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
         if (elect_one()) {
             uint32_t stage = 0, parity = 1, filled = 0;         // the first pass finds every slot empty
             bool ok = true;
+            const uint64_t policy = evict_first_policy();
             // channel tiles of a unit's K block; a unit's bytes are announced with them
             auto load_channels = [&](const IgUnit &un, uint32_t kb, uint32_t at) {
                 const uint32_t boxes = (un.count + kIgBoxRows - 1u) / kIgBoxRows, slot = ring + at * stage_bytes;
                 const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : SUBS * 128u);
                 mbar_expect_tx(&s.full[at], SUBS * kIgTileBytes + boxes * kIgBoxRows * 128u);
-                tma_load_2d(slot, &args.b, kb * 128u, ch0, &s.full[at]);
-                if (SUBS == 2) tma_load_2d(slot + kIgTileBytes, &args.b, kb * 128u, GATED ? ch0 + p.n : ch0 + 128u, &s.full[at]);
+#pragma unroll
+                for (uint32_t t = 0; t < SUBS; ++t) {
+                    const uint32_t ch = ch0 + t * (GATED ? p.n : 128u);
+                    if (p.evict_first) tma_load_2d_once(slot + t * kIgTileBytes, &args.b, kb * 128u, ch, &s.full[at], policy);
+                    else tma_load_2d(slot + t * kIgTileBytes, &args.b, kb * 128u, ch, &s.full[at]);
+                }
             };
             uint32_t early = 0;                                  // K blocks whose channels are on their way before the rows can be
             if (p.ready && blockIdx.x < total) {
