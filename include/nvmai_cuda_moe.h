@@ -513,7 +513,8 @@ NVMAI_API int nvmai_cuda_moe_quantize_rows(const void *x, uint32_t elem, uint32_
  * are expert e's, rows of none are left as they were; NULL with num_experts = 1: all rows.
  * a: codes with a_scales (NVMAI_ELEM_I8), or F16 / F32 / BF16 rows with a_scales = NULL, which the call
  * quantises as quantize_rows does; these need a workspace of _int8_matmul_workspace bytes.
- * Codes start on 16-byte boundaries and their strides are multiples of 16.  k < 131072 (the sum fits 32 bits);
+ * Rows of codes start on 16-byte boundaries, their strides are multiples of 16, and they are readable to the next
+ * multiple of 16 bytes (what is there does not matter).  k < 131072 (the sum fits 32 bits);
  * rows = 0 is valid.  The bits of a row's output do not depend on the rows beside it.  A bounded
  * device-side wait that gives up is reported by nvmai_cuda_moe_int8_matmul_status. */
 NVMAI_API uint64_t nvmai_cuda_moe_int8_matmul_workspace(uint32_t rows, uint32_t k, uint32_t a_elem);

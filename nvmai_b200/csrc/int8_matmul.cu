@@ -69,37 +69,44 @@ constexpr uint32_t kSms = 148;
 
 struct IgTile { uint32_t subs, nt; };
 
-// Rows of a unit where the rows are spread over experts.  An expert's codes come once for each of its units (past the first from
-// the L2), so a unit holds the average expert and 2.5 times the spread of an even routing around it.  Past 128 rows
-// that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 118.0 us, 160 110.5,
-// 192 113.7 (three ring slots instead of four); 512 -> 2048: 72.6, 69.7, 67.7.  Two channel tiles a unit read the rows half
-// as often: 201 tokens, 512 -> 2048, 54.1 us with one, 46.7 with two.
-IgTile grouped_tile(const Matmul &m) {
-    const float average = (float)m.rows / (float)m.E;
-    const uint32_t want = (uint32_t)std::ceil((average + 2.5f * std::sqrt(average)) / 32.0f) * 32u;
-    return IgTile{m.act != kActNone || m.n > 128 ? 2u : 1u, std::min(160u, std::max(32u, want))};
-}
+// Features of a unit.
+uint32_t unit_features(const Matmul &m, uint32_t subs) { return m.act != kActNone ? 128 : 128 * subs; }
 
-// One matrix: the cheapest tile by a model of the time, in ns, fitted to 16 shapes (40 to 16384 rows, 512 to 2048 codes, 300 to 2048
-// channels): a K block costs 104 and 4.1 for each KB of it, the last epilogue of a block 10 for each row and tile of its unit (an
-// activation counts double), earlier ones 6.5 beside the next unit or, with one set of accumulators, 10 in its way.  The
-// tile it picks took at most 9 % longer than the best one in those shapes, 128 rows of two tiles up to 80 %.
-IgTile dense_tile(const Matmul &m) {
+// The cheapest tile for `experts` runs of `rows` rows by a model of the time, in ns, fitted to 16 shapes of one matrix (40 to 16384
+// rows, 512 to 2048 codes, 300 to 2048 channels): a K block costs 104 and 4.1 for each KB of it, the last epilogue of a block 10 for
+// each row and tile of its unit (an activation counts double), earlier ones 6.5 beside the next unit or, with one set of
+// accumulators, 10 in its way.  The tile it picks took at most 9 % longer than the best one in those shapes, 128 rows of two
+// tiles up to 80 %.
+IgTile cheapest_tile(const Matmul &m, uint32_t experts, float rows) {
     const bool gated = m.act != kActNone;
     const float blocks = (float)((m.k + 127) / 128);
     IgTile best{};
     float best_ns = INFINITY;
     for (uint32_t subs = gated ? 2 : 1; subs <= 2; ++subs)
         for (uint32_t nt = 32; nt * subs <= 512 && nt <= 256; nt += 32) {
-            const uint64_t tiles = (m.rows + nt - 1) / nt, units = tiles * ((m.n + (gated ? 128 : 128 * subs) - 1) / (gated ? 128 : 128 * subs));
-            const float waves = (float)((units + kSms - 1) / kSms), per = (float)(((m.rows + tiles - 1) / tiles + 15) / 16 * 16);
+            const float tiles = std::ceil(rows / (float)nt), units = tiles * (float)experts * (float)((m.n + unit_features(m, subs) - 1) / unit_features(m, subs));
+            const float waves = std::ceil(units / (float)kSms), per = std::ceil(rows / tiles / 16.0f) * 16.0f;
             const float kb = (float)(16 * subs) + std::ceil(per / 32.0f) * 4.0f, outs = per * (float)(subs * (gated ? 2 : 1));
             const float epilogues = 2 * subs * nt <= 512 ? 10.4f + 6.5f * (waves - 1.0f) : 10.4f * waves;
             const float ns = waves * blocks * (104.0f + 4.1f * kb) + outs * epilogues;
             if (ns < best_ns) { best_ns = ns; best = IgTile{subs, nt}; }
-            if (nt >= m.rows) break;
+            if ((float)nt >= rows) break;
         }
     return best;
+}
+
+// One matrix, or one for each expert.  Where every SM has several units HBM is the limit: the codes come once for each unit of an
+// expert (past the first from the L2), so a unit holds the average expert and 2.5 times the spread of an even routing around
+// it (the model takes twice).  Past 128 rows that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 118.0
+// us, 160 110.5, 192 113.7 (three ring slots instead of four); 512 -> 2048: 72.6, 69.7, 67.7.  Two channel tiles a unit read
+// the rows half as often: 201 tokens, 512 -> 2048, 54.1 us with one, 46.7 with two.
+IgTile row_tile(const Matmul &m) {
+    if (m.begin == nullptr) return cheapest_tile(m, 1, (float)m.rows);
+    const float average = (float)m.rows / (float)m.E;
+    const uint32_t want = (uint32_t)std::ceil((average + 2.5f * std::sqrt(average)) / 32.0f) * 32u;
+    const IgTile tile{m.act != kActNone || m.n > 128 ? 2u : 1u, std::min(160u, std::max(32u, want))};
+    const float units = std::ceil(average / (float)tile.nt) * (float)m.E * (float)((m.n + unit_features(m, tile.subs) - 1) / unit_features(m, tile.subs));
+    return units >= 3.0f * (float)kSms ? tile : cheapest_tile(m, m.E, std::max(1.0f, average + 2.0f * std::sqrt(average)));
 }
 
 cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
@@ -112,10 +119,10 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     p.status = status_word();
     if (!p.status || !code_map(&args.a, m.a, m.rows, m.k, m.a_stride, kIgBoxRows) ||
         !code_map(&args.b, m.b, (uint64_t)m.E * m.channels, m.k, m.b_stride, 128)) return cudaErrorInvalidValue;
-    const IgTile tile = m.begin != nullptr ? grouped_tile(m) : dense_tile(m);
+    const IgTile tile = row_tile(m);
     const uint32_t subs = tile.subs;
     p.nt = tile.nt;
-    p.channel_tiles = (m.n + (gated ? 128 : subs * 128) - 1) / (gated ? 128 : subs * 128);
+    p.channel_tiles = (m.n + unit_features(m, subs) - 1) / unit_features(m, subs);
     const size_t stage = subs * kIgTileBytes + (size_t)p.nt * 128;
     p.accs = 2 * subs * p.nt <= 512 ? 2 : 1;
     p.ready = m.ready;

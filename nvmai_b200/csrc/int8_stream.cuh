@@ -45,12 +45,16 @@ __device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 codes of a channel from position i on; what is behind k reads as 0 and is not touched
+// 16 codes of a row from position i < k on, those behind k as zeros.  Rows start on 16-byte boundaries and are readable to the next one,
+// so a row's last piece is fetched whole.
 __device__ __forceinline__ uint4 codes16(const int8_t *row, uint32_t i, uint32_t k) {
-    if (i + 16u <= k) return ldg_stream_u4(row + i);
-    uint32_t w[4] = {0, 0, 0, 0};
-    for (uint32_t j = 0; i + j < k; ++j) w[j / 4] |= (uint32_t)(uint8_t)row[i + j] << (8 * (j % 4));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    uint4 v = ldg_stream_u4(row + i);
+    if (i + 16u > k) {
+        const uint32_t n = k - i;                              // 1 .. 15 of them
+        auto keep = [n](uint32_t w, uint32_t at) { return n >= at + 4u ? w : n <= at ? 0u : w & (0xffffffffu >> (32u - 8u * (n - at))); };
+        v = make_uint4(keep(v.x, 0u), keep(v.y, 4u), keep(v.z, 8u), keep(v.w, 12u));
+    }
+    return v;
 }
 
 // T: type of the rows (int8_t: codes with a_scales).  V: elements of a row read at once.
@@ -106,20 +110,15 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
     const int8_t *b0 = p.b + ((size_t)e * p.channels + (live0 ? c0 : 0u)) * p.b_stride;
     const int8_t *b1 = p.b + ((size_t)e * p.channels + (live1 ? c1 : 0u)) * p.b_stride;
     const uint32_t steps = (p.k + kIsStep - 1u) / kIsStep;
-    const bool whole = p.k % 16u == 0u;                        // no piece of 16 codes ends inside
     uint4 w0[kIsAhead], w1[kIsAhead];
     auto request = [&](uint32_t s0) {
 #pragma unroll
         for (uint32_t i = 0; i < kIsAhead; ++i) {
             const uint32_t s = s0 + i * parts, at = s * kIsStep + t * 16u;
+            // behind k a channel's codes meet zeros of the rows, so its last piece needs no mask
             w0[i] = w1[i] = make_uint4(0, 0, 0, 0);
-            if (whole) {
-                if (at < p.k && live0) w0[i] = ldg_stream_u4(b0 + at);
-                if (at < p.k && live1) w1[i] = ldg_stream_u4(b1 + at);
-            } else if (s < steps) {
-                if (live0) w0[i] = codes16(b0, at, p.k);
-                if (live1) w1[i] = codes16(b1, at, p.k);
-            }
+            if (at < p.k && live0) w0[i] = ldg_stream_u4(b0 + at);
+            if (at < p.k && live1) w1[i] = ldg_stream_u4(b1 + at);
         }
     };
     request(part);
