@@ -30,11 +30,12 @@ struct IgParams {
     uint32_t ready;                      // the kernel in front made the rows' codes and nothing else that is read here
     uint32_t paired;                     // 16-bit outputs: two neighbouring channels go out in one store
     uint32_t channel_tiles;              // units across the channels
+    uint32_t box_channels;               // rows of a box of the matrix: 128, or what a narrower matrix has (lanes past it are not stored)
     unsigned int *status;
     uint32_t debug_drop_rows;            // test hook: block 0 leaves out the rows of its second K block, so waits run out
 };
 struct alignas(64) IgArgs {
-    CUtensorMap a, b;                    // [rows][k], [E * channels][k] bytes; boxes of 32 and of 128 rows x 128 bytes
+    CUtensorMap a, b;                    // [rows][k], [E * channels][k] bytes; boxes of 32 and of box_channels rows x 128 bytes
     IgParams p;
 };
 
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
             auto load_channels = [&](const IgUnit &un, uint32_t kb, uint32_t at) {
                 const uint32_t boxes = (un.count + kIgBoxRows - 1u) / kIgBoxRows, slot = ring + at * stage_bytes;
                 const uint32_t ch0 = un.e * p.channels + un.ch * (GATED ? 128u : SUBS * 128u);
-                mbar_expect_tx(&s.full[at], SUBS * kIgTileBytes + boxes * kIgBoxRows * 128u);
+                mbar_expect_tx(&s.full[at], (SUBS * p.box_channels + boxes * kIgBoxRows) * 128u);
 #pragma unroll
                 for (uint32_t t = 0; t < SUBS; ++t) {
                     const uint32_t ch = ch0 + t * (GATED ? p.n : 128u);

@@ -97,9 +97,11 @@ IgTile cheapest_tile(const Matmul &m, uint32_t experts, float rows) {
 
 // One matrix, or one for each expert.  Where every SM has several units HBM is the limit: the codes come once for each unit of an
 // expert (past the first from the L2), so a unit holds the average expert and 2.5 times the spread of an even routing around
-// it (the model takes twice).  Past 128 rows that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 118.0
-// us, 160 110.5, 192 113.7 (three ring slots instead of four); 512 -> 2048: 72.6, 69.7, 67.7.  Two channel tiles a unit read
-// the rows half as often: 201 tokens, 512 -> 2048, 54.1 us with one, 46.7 with two.
+// it.  Past 128 rows that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 118.0 us, 160
+// 110.5, 192 113.7 (three ring slots instead of four); 512 -> 2048: 72.6, 69.7, 67.7.  Two channel tiles a unit read the rows half
+// as often: 201 tokens, 512 -> 2048, 54.1 us with one, 46.7 with two.  Below three units an SM the model picks, for the average
+// and twice the spread: 41 tokens x 8 through 8 experts of 1711 -> 596 12.3 us with the rule above, 9.0 with the model; 201 x 8
+// through 16 of 2048 -> 2 x 512 14.1 / 12.2; 1000 x 8 through 64 of those 31.9 / 32.1.
 IgTile row_tile(const Matmul &m) {
     if (m.begin == nullptr) return cheapest_tile(m, 1, (float)m.rows);
     const float average = (float)m.rows / (float)m.E;
@@ -117,8 +119,10 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     p.rows = m.rows; p.k = m.k; p.n = m.n; p.channels = m.channels; p.E = m.E; p.begin = m.begin;
     p.a_scales = m.a_scales; p.b_scales = m.b_scales; p.act = m.act; p.out = m.out; p.out_stride = m.out_stride;
     p.status = status_word();
+    // a matrix of fewer than 128 features fetches no more rows than it has: 176 rows of 1161 -> 2 x 21 by 83 experts 9.6 -> 8.2 us
+    p.box_channels = std::min(128u, (m.n + 7) / 8 * 8);
     if (!p.status || !code_map(&args.a, m.a, m.rows, m.k, m.a_stride, kIgBoxRows) ||
-        !code_map(&args.b, m.b, (uint64_t)m.E * m.channels, m.k, m.b_stride, 128)) return cudaErrorInvalidValue;
+        !code_map(&args.b, m.b, (uint64_t)m.E * m.channels, m.k, m.b_stride, p.box_channels)) return cudaErrorInvalidValue;
     const IgTile tile = row_tile(m);
     const uint32_t subs = tile.subs;
     p.nt = tile.nt;
@@ -166,9 +170,10 @@ cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
     IsParams p{m.a, m.a_stride, m.a_scales, m.rows, m.k, m.b, m.b_stride, m.b_scales, m.n, m.channels, m.E, m.begin, m.act,
                m.out, m.out_elem, m.out_stride, m.ready, is_row_bytes(m.k), 1};
     const uint32_t steps = (m.k + kIsStep - 1) / kIsStep, columns = m.begin != nullptr ? m.rows : (m.rows + 8 * nt - 1) / (8 * nt);
-    auto blocks = [&] { return (m.n * p.parts + (gated ? 8 : 16) * kIsWarps - 1) / ((gated ? 8 : 16) * kIsWarps); };    // across the features
+    const uint32_t features = (gated ? 8 : 16) * kIsWarps;                // of a block whose warps do not split K
+    auto blocks = [&] { return (uint32_t)(((uint64_t)m.n * p.parts + features - 1) / features); };
     const uint64_t resident = nt == 1 ? 2 * kSms : kSms;                 // blocks
-    while (p.parts < kIsWarps && p.parts < steps && (steps > p.parts * kIsAhead || 2 * (uint64_t)blocks() * columns <= resident)) p.parts *= 2;
+    while (p.parts < kIsWarps && p.parts < steps && (steps > p.parts * kIsAhead || 2ull * blocks() * columns <= resident)) p.parts *= 2;
     const dim3 grid(blocks(), columns);
     auto go = [&](auto T, auto V, auto G, auto N) {
         return launch_pdl(int8_stream_kernel<decltype(T), decltype(V)::value, decltype(G)::value, decltype(N)::value>, grid,
