@@ -18,6 +18,8 @@ constexpr uint32_t kIgMaxStages = 8, kIgBoxRows = 32;
 constexpr uint32_t kIgTileBytes = 128 * 128;           // 128 channels x 128 codes
 constexpr uint32_t kActNone = 2;
 
+static __device__ unsigned int g_int8_status;      // a bounded wait gave up (nvmai_cuda_moe_int8_matmul_status)
+
 struct IgParams {
     uint32_t rows, k, n, channels, E;
     const uint32_t *begin;               // first row of each expert, or nullptr: one matrix
@@ -31,7 +33,6 @@ struct IgParams {
     uint32_t paired;                     // 16-bit outputs: two neighbouring channels go out in one store
     uint32_t channel_tiles;              // units across the channels
     uint32_t box_channels;               // rows of a box of the matrix: 128, or what a narrower matrix has (lanes past it are not stored)
-    unsigned int *status;
     uint32_t debug_drop_rows;            // test hook: block 0 leaves out the rows of its second K block, so waits run out
 };
 struct alignas(64) IgArgs {
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
             if (global_timer_ns() - t0 > limit) break;
         }
         *reinterpret_cast<volatile uint32_t *>(&s.gave_up) = 1u;
-        atomicExch(p.status, 1u);
+        atomicExch(&g_int8_status, 1u);
         return false;
     };
 

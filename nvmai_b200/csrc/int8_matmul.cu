@@ -37,8 +37,6 @@ struct Matmul {
 size_t code_stride(uint32_t k) { return ((size_t)k + 15) & ~(size_t)15; }
 size_t scales_offset(uint32_t rows, uint32_t k) { return ((size_t)rows * code_stride(k) + 255) & ~(size_t)255; }
 
-static __device__ unsigned int g_int8_status;      // a bounded wait gave up (nvmai_cuda_moe_int8_matmul_status)
-
 // One tensor map of rows of codes in boxes of `box_rows` rows x 128 bytes, 128-byte swizzle; bytes outside read as zeros.
 bool code_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t k, uint64_t stride, uint32_t box_rows) {
     const EncodeTiledFn enc = encode_tiled_fn();
@@ -49,20 +47,6 @@ bool code_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t k, uin
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The status word's address on the current device.
-unsigned int *status_word() {
-    static std::atomic<unsigned int *> at[64] = {};
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    unsigned int *known = at[dev].load(std::memory_order_acquire);
-    if (known == nullptr) {
-        void *p = nullptr;
-        if (cudaGetSymbolAddress(&p, g_int8_status) != cudaSuccess) { cudaGetLastError(); return nullptr; }
-        known = static_cast<unsigned int *>(p);
-        at[dev].store(known, std::memory_order_release);
-    }
-    return known;
-}
 std::atomic<bool> g_drop_copy{false};      // test hook, see nvmai_cuda_moe_debug_drop_int8_copy
 
 constexpr uint32_t kSms = 148;
@@ -118,10 +102,9 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
     const bool gated = m.act != kActNone;
     p.rows = m.rows; p.k = m.k; p.n = m.n; p.channels = m.channels; p.E = m.E; p.begin = m.begin;
     p.a_scales = m.a_scales; p.b_scales = m.b_scales; p.act = m.act; p.out = m.out; p.out_stride = m.out_stride;
-    p.status = status_word();
     // a matrix of fewer than 128 features fetches no more rows than it has: 176 rows of 1161 -> 2 x 21 by 83 experts 9.6 -> 8.2 us
     p.box_channels = std::min(128u, (m.n + 7) / 8 * 8);
-    if (!p.status || !code_map(&args.a, m.a, m.rows, m.k, m.a_stride, kIgBoxRows) ||
+    if (!code_map(&args.a, m.a, m.rows, m.k, m.a_stride, kIgBoxRows) ||
         !code_map(&args.b, m.b, (uint64_t)m.E * m.channels, m.k, m.b_stride, p.box_channels)) return cudaErrorInvalidValue;
     const IgTile tile = row_tile(m);
     const uint32_t subs = tile.subs;

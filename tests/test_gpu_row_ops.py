@@ -777,6 +777,53 @@ def test_status_refuses_a_capture():
     torch.cuda.synchronize()
 
 
+FIRST_CALLS = """
+import torch, nvmai_b200 as nv
+from nvmai_b200 import format as fmt
+t, k, e, d, n = 300, 4, 8, 128, 64
+dev = dict(device="cuda")
+g = torch.Generator(**dev).manual_seed(1)
+idx = torch.randint(0, e, (t, k), generator=g, **dev).to(torch.int32)
+x = torch.randn((t, d), generator=g, **dev)
+b = torch.randint(-127, 128, (e * n, d), generator=g, dtype=torch.int8, **dev)
+bs = torch.rand(e * n, generator=g, **dev)
+i32 = lambda *s: torch.empty(s, dtype=torch.int32, **dev)
+position, source, begin = i32(t, k), i32(t * k), i32(e + 1)
+rows, out, y, dw = torch.zeros(t * k, d, **dev), torch.empty(t * k, n, **dev), torch.empty(t, n, **dev), torch.empty(t, k, **dev)
+drows = torch.empty(t * k, n, **dev)
+work = torch.empty(nv.int8_matmul_workspace(t * k, d, fmt.ELEM_F32), dtype=torch.uint8, **dev)
+stream = torch.cuda.Stream()
+def run():
+    nv.sort_rows(idx, t, k, e, position, source, begin, x=x, d=d, elem=fmt.ELEM_F32, rows=rows, stream=stream)
+    nv.int8_matmul(rows, b, bs, out, t * k, d, n, a_elem=fmt.ELEM_F32, num_experts=e, expert_begin=begin, out_elem=fmt.ELEM_F32,
+                   workspace=work, workspace_bytes=work.numel(), stream=stream)
+    nv.merge_rows(out, t * k, position, t, k, n, y, elem=fmt.ELEM_F32, stream=stream)
+    nv.merge_rows_grad(y, out, t * k, position, None, t, k, n, drows, dw, elem=fmt.ELEM_F32, stream=stream)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    run()
+graph.replay()
+torch.cuda.synchronize()
+first = [v.clone() for v in (position, out, y, drows, dw)]
+for v in (out, y, drows, dw):
+    v.zero_()
+torch.cuda.synchronize()
+run()
+nv.int8_matmul_status(stream)
+assert all(torch.equal(a, b) for a, b in zip(first, (position, out, y, drows, dw)))
+print("the same")
+"""
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("pinned", [False, True])
 def test_buffers_of_the_host_are_refused(pinned):
     host, dev = torch.zeros(64, dtype=torch.float32, pin_memory=pinned), torch.zeros(64, device="cuda")
