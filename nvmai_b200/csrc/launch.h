@@ -42,7 +42,8 @@ inline cudaError_t ensure_smem(Kern kern, size_t bytes) {
 //      are visible, as soon as a kernel has started at all; the kernel in front itself is complete behind pdl_wait.
 //   2. A kernel that puts its own wait off may read, until then, only what kernels before the one in front wrote, and
 //      write only what none of them and not the one in front touches: the router GEMM beside the packing of the rows
-//      (batch_rows.cuh), a streaming kernel beside the grouped GEMM of the same phase (SgParams::beside).
+//      (batch_rows.cuh), a streaming kernel beside the grouped GEMM of the same phase (SgParams::beside), the 8-bit products beside
+//      the quantisation of their rows (IgParams::ready, IsParams::ready).
 //      Weights and the work list ahead of the wait (list_ready in batch_path.h) are of this kind.  Tagged words are the exception:
 //      stage 3 polls what stage 2 writes (Handover in staged_decode.cuh).
 // A kernel that lets its dependents start without having waited would break both without any sign of it.

@@ -32,12 +32,6 @@ __device__ __forceinline__ void store_elem(void *p, uint32_t elem, size_t i, flo
 // V neighbouring elements, moved in one access (V * sizeof(T) <= 16 bytes, aligned to that)
 template <typename T, int V> struct alignas(sizeof(T) * V) Piece { T v[V]; };
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
 // ---- symmetric 8-bit codes of a row (nvmai_cuda_moe_quantize_rows) ----------------------------------------
 // Every step is one rounding to fp32, so any order of the elements gives the same codes.  kTinyRow: below it 127 / m would
 // overflow.  An infinite or NaN m: codes of 0 and a scale of NaN.
