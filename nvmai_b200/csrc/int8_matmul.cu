@@ -142,10 +142,10 @@ uint32_t stream_tiles(const Matmul &m) {
     const uint32_t nt = m.begin != nullptr || m.rows <= 8 ? 1 : m.rows <= 16 ? 2 : 4;
     return is_smem(m.k, nt) <= 200 * 1024 ? nt : 0;
 }
-// Does it quantise the rows itself?  Each of its blocks then does, 0.5 us a row in front of the product; a launch for all of
-// them runs beside the fetching of the codes, and costs the host 2.4 us (2048 -> 2 x 512, one launch / two: 1 row 3.8 / 4.3 us, 2
-// rows 4.5 / 4.1, 4 rows 5.6 / 4.1; one token through eight experts 7.9 / 7.4).
-bool stream_quantizes(const Matmul &m) { return m.begin != nullptr || m.rows <= 2; }
+// Does it quantise the rows itself?  Each of its blocks then does, 0.3 us a row of 2048 in front of the product; a launch for all of
+// them runs beside the fetching of the codes, and costs the host 2.4 us (2048 -> 2 x 512, one launch / two: 1 row 3.7 / 4.3 us, 3
+// rows 4.3 / 4.3, 4 rows 4.8 / 4.3; 3 rows of 4096 6.5 / 5.0; one token through eight experts 7.3 / 7.4).
+bool stream_quantizes(const Matmul &m) { return m.begin != nullptr || (m.rows <= 4 && m.rows * m.k <= 6144); }
 
 cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
     using std::integral_constant;
@@ -162,9 +162,13 @@ cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {
         return launch_pdl(int8_stream_kernel<decltype(T), decltype(V)::value, decltype(G)::value, decltype(N)::value>, grid,
                           dim3(kIsThreads), is_smem(m.k, nt), st, true, p);
     };
+    // rows that the kernel quantises itself are eight a block at most (stream_quantizes)
     auto with_tiles = [&](auto T, auto V, auto G) {
-        return nt == 1 ? go(T, V, G, integral_constant<int, 1>{}) : nt == 2 ? go(T, V, G, integral_constant<int, 2>{})
-                                                                           : go(T, V, G, integral_constant<int, 4>{});
+        if constexpr (sizeof(T) == 1) {
+            if (nt == 2) return go(T, V, G, integral_constant<int, 2>{});
+            if (nt == 4) return go(T, V, G, integral_constant<int, 4>{});
+        }
+        return go(T, V, G, integral_constant<int, 1>{});
     };
     auto with_gate = [&](auto T, auto V) {
         return gated ? with_tiles(T, V, integral_constant<bool, true>{}) : with_tiles(T, V, integral_constant<bool, false>{});

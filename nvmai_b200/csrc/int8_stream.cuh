@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
     constexpr bool kCoded = sizeof(T) == 1;
     constexpr uint32_t kRows = 8 * NT, kFeatures = GATED ? 8 : 16;
     extern __shared__ __align__(16) unsigned char is_smem_raw[];
-    __shared__ float scale[kRows];
+    __shared__ float scale[kRows], inverse[kRows];
     __shared__ uint32_t top[kRows], found[3];
     unsigned char *codes = is_smem_raw;
     int *partial = reinterpret_cast<int *>(is_smem_raw + (size_t)p.row_bytes * kRows);
@@ -140,42 +140,47 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
             for (int x = 0; x < V; ++x) m = max(m, magnitude_bits(elem_to_float(v.v[x])));
             return m;
         };
-        for (uint32_t r0 = 0; r0 < count; r0 += 4u) {          // four rows' pieces on their way at a time
-            uint32_t m[4] = {0, 0, 0, 0};
-            for (uint32_t i = tid; i < pieces; i += kIsThreads) {
-                P v[4];
+        // the first piece of up to four rows stays in registers; what else there is comes twice, the second time from the L1
+        auto piece = [&](uint32_t r, uint32_t i) { return reinterpret_cast<const P *>(a + (size_t)r * p.a_stride)[i]; };
+        constexpr uint32_t kHeld = 4;
+        P held[kHeld];
+        held[0] = early;
 #pragma unroll
-                for (uint32_t x = 0; x < 4u; ++x)
-                    if (r0 + x < count) v[x] = r0 + x == 0u && i == tid ? early : reinterpret_cast<const P *>(a + (size_t)(r0 + x) * p.a_stride)[i];
+        for (uint32_t r = 1; r < kHeld; ++r)
+            if (r < count && tid < pieces) held[r] = piece(r, tid);
+        auto maximum = [&](uint32_t r, uint32_t m, uint32_t from) {
+            for (uint32_t i = from; i < pieces; i += kIsThreads) m = largest(piece(r, i), m);
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) atomicMax(&top[r], m);
+        };
 #pragma unroll
-                for (uint32_t x = 0; x < 4u; ++x)
-                    if (r0 + x < count) m[x] = largest(v[x], m[x]);
-            }
-#pragma unroll
-            for (uint32_t x = 0; x < 4u; ++x)
-                if (r0 + x < count) {
-                    m[x] = __reduce_max_sync(0xffffffffu, m[x]);
-                    if (lane == 0) atomicMax(&top[r0 + x], m[x]);
-                }
+        for (uint32_t r = 0; r < kHeld; ++r)
+            if (r < count) maximum(r, tid < pieces ? largest(held[r], 0u) : 0u, tid + kIsThreads);
+        for (uint32_t r = kHeld; r < count; ++r) maximum(r, 0u, tid);
+        __syncthreads();
+        if (tid < count) {
+            const RowScale rs = row_scale_bits(top[tid]);
+            scale[tid] = rs.scale;
+            inverse[tid] = rs.inverse;
         }
         __syncthreads();
-        for (uint32_t r = 0; r < count; ++r) {
-            const RowScale rs = row_scale_bits(top[r]);
-            if (tid == 0) scale[r] = rs.scale;
-            const P *src = reinterpret_cast<const P *>(a + (size_t)r * p.a_stride);
-            for (uint32_t i = tid; i < padded / V; i += kIsThreads) {
-                Q q;
-                if (i < pieces) {
-                    const P v = r == 0u && i == tid ? early : src[i];
+        auto store_codes = [&](uint32_t r, uint32_t i, const P &v) {
+            const RowScale rs{0.0f, inverse[r]};
+            Q q;
 #pragma unroll
-                    for (int x = 0; x < V; ++x) q.v[x] = row_code(elem_to_float(v.v[x]), rs);
-                } else {
+            for (int x = 0; x < V; ++x) q.v[x] = i < pieces ? row_code(elem_to_float(v.v[x]), rs) : (int8_t)0;
+            *reinterpret_cast<Q *>(codes + r * p.row_bytes + i * V) = q;
+        };
+        auto rest = [&](uint32_t r, uint32_t from) {
+            for (uint32_t i = from; i < padded / V; i += kIsThreads) store_codes(r, i, i < pieces ? piece(r, i) : P{});
+        };
 #pragma unroll
-                    for (int x = 0; x < V; ++x) q.v[x] = 0;
-                }
-                *reinterpret_cast<Q *>(codes + r * p.row_bytes + i * V) = q;
+        for (uint32_t r = 0; r < kHeld; ++r)
+            if (r < count) {
+                if (tid < padded / V) store_codes(r, tid, held[r]);
+                rest(r, tid + kIsThreads);
             }
-        }
+        for (uint32_t r = kHeld; r < count; ++r) rest(r, tid);
     }
     __syncthreads();
 
