@@ -19,7 +19,9 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // ---- sort_rows ------------------------------------------------------------------------------------------
 // A stable counting sort: the row of a pair is (kept pairs of smaller experts) + (pairs of its expert in front of it).  Each
 // block has a run of tokens; it counts the experts of all pairs, those in front of its run apart, and ranks its own pairs
-// with one warp, 32 at a time (__match_any_sync gives the pairs of the same expert).  Then its warps move the tokens' rows.
+// with one warp, 32 at a time (__match_any_sync gives the pairs of the same expert).  Then its warps move the tokens' rows.  Writing
+// bounds it: 4096 tokens of 4 KB to eight experts each take 32.3 us on a B200, 5.9 of them for the order (the same 134 MB written in order
+// take 24.6); one token 3.0.
 constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kSms = 148, kSortBlocks = kSms;
 constexpr uint32_t kSortOwn = 4096;          // most pairs of a block: their experts and rows are in shared memory
@@ -357,7 +359,8 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
     }
 }
 
-// Rows of 16-bit elements that share no 4-byte boundary: a thread sums every 32nd element, four of them and four slots at a time.
+// Rows of 16-bit elements that share no 4-byte boundary: a thread sums every 32nd element, four of them and four slots at a time
+// (two-byte accesses bound it: 1531 tokens of eight rows of 999 elements 14.4 us on a B200, 1.9 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) merge_narrow_kernel(MergeParams p) {
     constexpr int U = 4, kAhead = 4;
