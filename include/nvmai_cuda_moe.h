@@ -451,9 +451,10 @@ NVMAI_API int nvmai_cuda_moe_residual_add_f16(void *hidden, const void *delta, u
 /* ---- row operators: rows sorted by expert and back, products in 8-bit integers --------------
  * For hosts that run experts of their own between router and sum (other weights, adapters,
  * training of router and inputs), or experts stored as symmetric 8-bit integers.  No counterpart
- * in the reference.  No handle: every buffer is the caller's, nothing is allocated, no state is
- * kept between calls, and calls on different streams are independent as long as their buffers
- * (workspaces included) are.  Calls can be captured.  Strides count elements (codes: bytes) from
+ * in the reference.  No handle: every buffer is the caller's, nothing is allocated on the device,
+ * no state is kept between calls (but for the reports of int8_matmul_status), and calls on
+ * different streams are independent as long as their buffers (workspaces included) are.  Calls can
+ * be captured.  Strides count elements (codes: bytes) from
  * one row to the next and are at least the row's length.  All pointers are memory of the current
  * device, or managed memory (NVMAI_CUDA_EINVAL otherwise); indexes and positions are checked on
  * the device, an entry out of range counts as not held, never as an address.  Outputs overlap
@@ -525,7 +526,10 @@ NVMAI_API int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_
                                          uint32_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream);
 
 /* Waits for `stream`, then returns NVMAI_CUDA_ETIMEOUT if a bounded device-side wait of an int8_matmul call on the
- * current device gave up since the last call of this function (the outputs of that product are undefined), else 0.
+ * current device gave up that this function has not reported for this stream yet, else 0.  The outputs of that product are
+ * undefined.  It may be another stream's product: every stream is told of every one, at least once, so that no
+ * question takes away another stream's answer.  A stream is told of what came after its first int8_matmul
+ * call; one that never had such a call (it replays graphs captured elsewhere) of all since the process began.
  * NVMAI_CUDA_EINVAL on a stream that is being captured. */
 NVMAI_API int nvmai_cuda_moe_int8_matmul_status(void *stream);
 

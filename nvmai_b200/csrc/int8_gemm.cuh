@@ -20,7 +20,7 @@ constexpr uint32_t kIgMaxStages = 8, kIgBoxRows = 32;
 constexpr uint32_t kIgTileBytes = 128 * 128;           // 128 channels x 128 codes
 constexpr uint32_t kActNone = 2;
 
-static __device__ unsigned int g_int8_status;      // a bounded wait gave up (nvmai_cuda_moe_int8_matmul_status)
+static __device__ unsigned int g_int8_give_ups;    // bounded waits that ran out, never cleared (give_ups.h)
 
 struct IgParams {
     uint32_t rows, k, n, channels, E;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
             if (global_timer_ns() - t0 > limit) break;
         }
         *reinterpret_cast<volatile uint32_t *>(&s.gave_up) = 1u;
-        atomicExch(&g_int8_status, 1u);
+        atomicAdd(&g_int8_give_ups, 1u);
         return false;
     };
 

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "give_ups.h"
 #include "int8_gemm.cuh"
 #include "int8_stream.cuh"
 #include "launch.h"
@@ -48,6 +49,12 @@ bool code_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t k, uin
 }
 
 std::atomic<bool> g_drop_copy{false};      // test hook, see nvmai_cuda_moe_debug_drop_int8_copy
+
+// made with the first call and never destroyed: threads may still ask while the process ends
+GiveUps &give_ups() {
+    static GiveUps *all = new GiveUps;
+    return *all;
+}
 
 constexpr uint32_t kSms = 148;
 
@@ -211,7 +218,9 @@ int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride
             if (workspace_bytes < nvmai_cuda_moe_int8_matmul_workspace(rows, k, a_elem)) return NVMAI_CUDA_ERANGE;
             if (!workspace || !aligned_to(workspace, 16)) return NVMAI_CUDA_EINVAL;
         }
-        if (!on_current_device({a, a_scales, b, b_scales, expert_begin, out, coded ? nullptr : workspace})) return NVMAI_CUDA_EINVAL;
+        int dev = -1;
+        if (!on_current_device({a, a_scales, b, b_scales, expert_begin, out, coded ? nullptr : workspace}, &dev)) return NVMAI_CUDA_EINVAL;
+        give_ups().product(dev, stream);
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         Matmul m{a, a_elem, a_stride, a_scales, rows, k, static_cast<const int8_t *>(b), b_stride, b_scales, n, (uint32_t)channels,
                  num_experts, expert_begin, activation, out, out_elem, out_stride, false};
@@ -233,23 +242,20 @@ int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_t a_stride
 }
 
 int nvmai_cuda_moe_int8_matmul_status(void *stream) {
-    unsigned int status = 0;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(st, &capturing) != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
-    if (capturing != cudaStreamCaptureStatusNone) return NVMAI_CUDA_EINVAL;        // a capture has nothing to wait for
-    if (cudaMemcpyFromSymbolAsync(&status, g_int8_status, sizeof(status), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
-        cudaStreamSynchronize(st) != cudaSuccess) {
-        cudaGetLastError();
-        return NVMAI_CUDA_ECUDA;
-    }
-    if (status == 0) return NVMAI_CUDA_OK;
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(g_int8_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st) != cudaSuccess) {
-        cudaGetLastError();
-        return NVMAI_CUDA_ECUDA;
-    }
-    return NVMAI_CUDA_ETIMEOUT;
+    return without_exceptions([&]() -> int {
+        unsigned int count = 0;
+        int dev = -1;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaStreamIsCapturing(st, &capturing) != cudaSuccess) { cudaGetLastError(); return NVMAI_CUDA_ECUDA; }
+        if (capturing != cudaStreamCaptureStatusNone) return NVMAI_CUDA_EINVAL;        // a capture has nothing to wait for
+        if (cudaMemcpyFromSymbolAsync(&count, g_int8_give_ups, sizeof(count), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+            cudaStreamSynchronize(st) != cudaSuccess) {
+            cudaGetLastError();
+            return NVMAI_CUDA_ECUDA;
+        }
+        return give_ups().news(dev, stream, count) ? NVMAI_CUDA_ETIMEOUT : NVMAI_CUDA_OK;
+    });
 }
 
 int nvmai_cuda_moe_debug_drop_int8_copy(void) {

@@ -17,9 +17,10 @@ inline bool aligned_to(const void *p, size_t bytes) { return reinterpret_cast<ui
 // Every pointer given (null ones aside) is memory of the current device, or managed memory: a buffer of another device or of the
 // host would be an illegal address in the kernel.  An error is cleared: the call is refused, the context is as it was.
 // 0.05 us a pointer.
-inline bool on_current_device(std::initializer_list<const void *> ptrs) {
+inline bool on_current_device(std::initializer_list<const void *> ptrs, int *device = nullptr) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return false; }
+    if (device != nullptr) *device = dev;
     for (const void *p : ptrs) {
         if (p == nullptr) continue;
         cudaPointerAttributes a;

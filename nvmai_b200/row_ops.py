@@ -77,7 +77,8 @@ def int8_matmul(a, b, b_scales, out, rows: int, k: int, n: int, *, a_elem: int =
 
 
 def int8_matmul_status(stream=None) -> None:
-    """Waits for `stream`; raises NvmaiError(ETIMEOUT) if an `int8_matmul` call gave up a device-side wait."""
+    """Waits for `stream`; raises NvmaiError(ETIMEOUT) if an `int8_matmul` call on the device, on this stream or another, gave up
+    a device-side wait that this stream has not been told of."""
     check(_lib.lib().nvmai_cuda_moe_int8_matmul_status(_stream(stream)), "int8_matmul_status")
 
 
