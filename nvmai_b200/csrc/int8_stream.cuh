@@ -46,10 +46,18 @@ __device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 codes past the L1, by an ordinary load: rows, and a matrix that was just quantised too, may come from the kernel in front, which
+// still runs when the first blocks here start, and the non-coherent load is for memory that nobody writes while its kernel lives.
+__device__ __forceinline__ uint4 load_codes(const int8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // 16 codes of a row from position i < k on, those behind k as zeros.  Rows start on 16-byte boundaries and are readable to the next one,
 // so a row's last piece is fetched whole.
 __device__ __forceinline__ uint4 codes16(const int8_t *row, uint32_t i, uint32_t k) {
-    uint4 v = ldg_stream_u4(row + i);
+    uint4 v = load_codes(row + i);
     if (i + 16u > k) {
         const uint32_t n = k - i;                              // 1 .. 15 of them
         auto keep = [n](uint32_t w, uint32_t at) { return n >= at + 4u ? w : n <= at ? 0u : w & (0xffffffffu >> (32u - 8u * (n - at))); };
@@ -118,8 +126,8 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
             const uint32_t s = s0 + i * parts, at = s * kIsStep + t * 16u;
             // behind k a channel's codes meet zeros of the rows, so its last piece needs no mask
             w0[i] = w1[i] = make_uint4(0, 0, 0, 0);
-            if (at < p.k && live0) w0[i] = ldg_stream_u4(b0 + at);
-            if (at < p.k && live1) w1[i] = ldg_stream_u4(b1 + at);
+            if (at < p.k && live0) w0[i] = load_codes(b0 + at);
+            if (at < p.k && live1) w1[i] = load_codes(b1 + at);
         }
     };
     request(part);
