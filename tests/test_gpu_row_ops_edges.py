@@ -3,13 +3,14 @@ to do, activations in their tails, tile plans of large products, second turns of
 
 Tolerances as in test_gpu_row_ops.py: `U` = 2^-24 is half a step of fp32, `half_step(t)` the output type's."""
 
+import numpy as np
 import pytest
 import torch
 
 import nvmai_b200 as nv
 from nvmai_b200 import _lib
 from nvmai_b200 import format as fmt
-from test_gpu_row_ops import check_product, code_of, codes
+from test_gpu_row_ops import TYPES, U, check_product, code_of, codes, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +45,33 @@ def test_a_report_reaches_every_streams_owner():
         debug_set_wait_limit(0)
         for stream in (one, two, None):
             code_of(lambda: nv.int8_matmul_status(stream))
+
+
+# ---- activations in their tails ----------------------------------------------------------------------------------
+
+def tails(rows, first, scale, up, activation, out):
+    """rows of one code 1: gate values are -(first + j) * scale exactly, for j = 0 .. 47, up values are `up`.  -> output, gates"""
+    n, k = 48, 16
+    a = torch.zeros((rows, k), dtype=torch.int8, device="cuda")
+    a[:, 0] = 1
+    b = torch.zeros((2 * n, k), dtype=torch.int8, device="cuda")
+    b[:n, 0] = -(first + torch.arange(n, device="cuda")).to(torch.int8)
+    b[n:, 0] = 1
+    sb = torch.full((2 * n,), scale, device="cuda")
+    sb[n:] = up
+    t, elem = TYPES[out]
+    y = torch.empty((rows, n), dtype=t, device="cuda")
+    nv.int8_matmul(a, b, sb, y, rows, k, n, a_scales=torch.ones(rows, device="cuda"), activation=activation, out_elem=elem)
+    return y, b[:n, 0].double()[None, :] * scale
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("rows", [1, 8, 40])
+def test_silu_far_below_zero(rows, out):
+    """e^-g leaves fp32 below -88.7 while the gate times a large up row does not: 2^-149 is the step of fp32 below 2^-126, which e^g
+    is off by two of, and its product with g by half of one"""
+    up = float(np.float32(1e30))
+    y, g = tails(rows, 80, 1.0, up, fmt.ACT_SILU, out)
+    want = g * torch.exp(g) / (1 + torch.exp(g)) * up
+    tol = ((1 + g.abs()) * 3 + 11) * U * want.abs() * 1.01 + (2 * g.abs() + 1) * 2.0 ** -149 * up + half_step(TYPES[out][0], want) * 1.01
+    assert ((y.double() - want).abs() <= tol).all()
