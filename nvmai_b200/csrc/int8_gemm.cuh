@@ -72,23 +72,31 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-// The gate's activation.  SiLU as g / (1 + e^-g) above zero and g e^g / (1 + e^g) below, so that no e^ overflows: with the first form
-// alone everything below -88.7 would be 0, and times a large up row it is not.  HALF, for 16-bit outputs, takes the hardware's exp2
-// and reciprocal, whose error of (2 |g| + 9) 2^-24 (the argument's roundings, 2 ulp, 1 ulp and three more roundings) is at most
-// 0.013 of fp16's rounding and 0.002 of bf16's up to |g| = 50, 0.021 and 0.003 up to 80.  The exact division costs more than
-// the rest of an output.
+// The gate's activation: g / (1 + e^-z), which for SiLU has z = g, and for the tanh form of GELU, 0.5 g (1 + tanh y), z = 2 y (1 + tanh
+// itself keeps no digit of a value near 0: below g = -5.2 the result would be 0).  Below z = 0 as g / (1 + e^z) e^z, so that no e^
+// overflows: with the first form alone everything below -88.7 would be 0, and times a large up row it is not.
+// The hardware's exp2 and reciprocal have an error of (2 |z| + 9) 2^-24 (the argument's roundings, 2 ulp, 1 ulp and three more
+// roundings), at most 0.013 of fp16's rounding and 0.002 of bf16's up to |z| = 50, 0.021 and 0.003 up to 80; GELU's z is off by
+// 6 |z| 2^-24 before that.  So 16-bit outputs (HALF) and GELU take them; SiLU for fp32 outputs takes expf and the exact division,
+// which cost more than the rest of an output (GELU with them, 4096 tokens, fp32 out: 128 us).
+// Roundings are named where the compiler could fuse a product and a sum in one kernel and not in another: a row's bits
+// do not depend on the kernel.
 template <bool HALF>
 __device__ __forceinline__ float gate_act(float g, uint32_t act) {
-    if (act != ACT_SILU) return hidden_act(g, act);
-    if (HALF) {
-        float e, r;
-        asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.4426950408889634f));
-        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-        return (g < 0.0f ? g * e : g) * r;
+    const float z = act == ACT_SILU ? g : __fmul_rn(2.0f * 0.7978845608028654f, __fmaf_rn(0.044715f, __fmul_rn(__fmul_rn(g, g), g), g));
+    float e, q;
+    if (HALF || act != ACT_SILU) {
+        asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(fabsf(z), -1.4426950408889634f)));
+        asm("rcp.approx.f32 %0, %1;" : "=f"(q) : "f"(__fadd_rn(1.0f, e)));
+        q *= g;
+    } else {
+        e = expf(-fabsf(z));
+        q = g / __fadd_rn(1.0f, e);
     }
-    const float e = expf(-fabsf(g));
-    return (g < 0.0f ? g * e : g) / (1.0f + e);
+    return z < 0.0f ? q * e : q;
 }
+// value of a whole-number sum
+__device__ __forceinline__ float scaled(float sa, float sb, int sum) { return __fmul_rn(__fmul_rn(sa, sb), (float)sum); }
 
 // A box of the matrix whose lines are the first to leave the L2.
 __device__ __forceinline__ uint64_t evict_first_policy() {
@@ -365,13 +373,13 @@ __global__ void __launch_bounds__(kIgThreads, 1) int8_gemm_kernel(const __grid_c
                     if constexpr (GATED) {
 #pragma unroll
                         for (uint32_t k = 0; k < 16u; ++k)
-                            x[k] = gate_act<kHalf>((sa[k] * sb0) * (float)(int)v[r][0][k], p.act) * ((sa[k] * sb1) * (float)(int)v[r][1][k]);
+                            x[k] = gate_act<kHalf>(scaled(sa[k], sb0, (int)v[r][0][k]), p.act) * scaled(sa[k], sb1, (int)v[r][1][k]);
                         store(x, out, un.count - c, live0);
                     } else {
 #pragma unroll
                         for (uint32_t t = 0; t < SUBS; ++t) {
 #pragma unroll
-                            for (uint32_t k = 0; k < 16u; ++k) x[k] = (sa[k] * (t ? sb1 : sb0)) * (float)(int)v[r][t][k];
+                            for (uint32_t k = 0; k < 16u; ++k) x[k] = scaled(sa[k], t ? sb1 : sb0, (int)v[r][t][k]);
                             store(x, out + 128u * t, un.count - c, t ? live1 : live0);
                         }
                     }

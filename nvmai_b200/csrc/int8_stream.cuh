@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
             v += partial[w * NT * 128u + at];
             if (GATED) u += partial[w * NT * 128u + at + 2u];
         }
-        float x = (scale[r] * bs[jf]) * (float)v;
-        if (GATED) x = (p.out_elem == ELEM_F32 ? gate_act<false>(x, p.act) : gate_act<true>(x, p.act)) * ((scale[r] * bs[p.n + jf]) * (float)u);
+        float x = scaled(scale[r], bs[jf], v);
+        if (GATED) x = (p.out_elem == ELEM_F32 ? gate_act<false>(x, p.act) : gate_act<true>(x, p.act)) * scaled(scale[r], bs[p.n + jf], u);
         store_elem(p.out, p.out_elem, (size_t)(row0 + r) * p.out_stride + jf, x);
     }
 }

@@ -75,3 +75,47 @@ def test_silu_far_below_zero(rows, out):
     want = g * torch.exp(g) / (1 + torch.exp(g)) * up
     tol = ((1 + g.abs()) * 3 + 11) * U * want.abs() * 1.01 + (2 * g.abs() + 1) * 2.0 ** -149 * up + half_step(TYPES[out][0], want) * 1.01
     assert ((y.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("rows", [1, 8, 40])
+@pytest.mark.parametrize("first", [0, 48, 80])
+def test_gelu_far_below_zero(rows, out, first):
+    """0.5 g (1 + tanh y) = g / (1 + e^-2y).  y: two constants, a cube of two steps, a fused step and a product are 6 roundings; with
+    the argument's for exp2 8 |2 y| U of e^2y, and 12 U for exp, sum, quotient and products.  Below 2^-126 e^2y
+    is off by two steps of 2^-149 and its product with g by half of one"""
+    y, g = tails(rows, first, 0.125, 1.0, fmt.ACT_GELU_TANH, out)
+    z = 2 * 0.7978845608028654 * (g + 0.044715 * g ** 3)
+    want = g * torch.exp(z) / (1 + torch.exp(z))
+    tol = (8 * z.abs() + 12) * U * want.abs() * 1.01 + (2 * g.abs() + 1) * 2.0 ** -149 + half_step(TYPES[out][0], want) * 1.01
+    assert ((y.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+def test_gelu_of_large_gates(rows, out):
+    """far above zero the gate itself (its product and the up row's: two roundings), far below it nothing"""
+    up = float(np.float32(1e-30))
+    for scale in (1e20, -1e20, 1e30, -1e30):
+        y, g = tails(rows, 1, float(np.float32(scale)), up, fmt.ACT_GELU_TANH, out)
+        want = g.clamp(min=0) * up
+        assert ((y.double() - want).abs() <= 2 * U * want * 1.01 + half_step(TYPES[out][0], want) * 1.01).all()
+
+
+@pytest.mark.parametrize("k,n", [(512, 136), (2048, 24), (700, 33)])
+def test_gelu_has_the_same_bits_in_every_kernel(k, n):
+    most = 200
+    a, sa = codes(171, most, k)
+    b, sb = codes(172, 2 * n, k)
+    sb = sb * (0.5 / (k ** 0.5 * 74 * 74))
+    for t, elem in TYPES.values():
+        def run(rows, experts=1, begin=None):
+            y = torch.empty((rows, n), dtype=t, device="cuda")
+            nv.int8_matmul(a, b.repeat(experts, 1), sb.repeat(experts), y, rows, k, n, a_scales=sa, a_stride=a.shape[1], b_stride=b.shape[1],
+                           num_experts=experts, expert_begin=begin, activation=fmt.ACT_GELU_TANH, out_elem=elem)
+            return y
+        whole = run(most)
+        for rows in (1, 7, 16, 31, 32, 33, 100):
+            assert torch.equal(run(rows), whole[:rows]), rows
+        begin = torch.tensor([0, 3, 3, 60, most], dtype=torch.int32, device="cuda")
+        assert torch.equal(run(most, 4, begin), whole)
