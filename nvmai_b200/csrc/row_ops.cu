@@ -592,6 +592,7 @@ int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uint32_t top_
                              void *rows, uint32_t rows_elem, uint32_t rows_stride, float *row_scales, void *workspace,
                              uint64_t workspace_bytes, void *stream) {
     return without_exceptions([&]() -> int {
+        if (tokens == 0) x = rows = row_scales = nullptr;            // buffers of no rows have no address, whatever the others are
         if (!expert_begin || (tokens != 0 && (!idx || !position || !source))) return NVMAI_CUDA_EINVAL;
         if (top_k == 0 || top_k > kRowMaxTopK || num_experts == 0 || num_experts > kRowMaxExperts) return NVMAI_CUDA_ERANGE;
         if ((uint64_t)tokens * top_k >= (1ull << 26)) return NVMAI_CUDA_ERANGE;

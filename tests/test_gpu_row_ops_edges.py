@@ -47,6 +47,23 @@ def test_a_report_reaches_every_streams_owner():
             code_of(lambda: nv.int8_matmul_status(stream))
 
 
+# ---- calls with nothing to do ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows_elem", [fmt.ELEM_F16, fmt.ELEM_I8])
+@pytest.mark.parametrize("sized", [False, True])
+def test_sorting_no_tokens_writes_empty_experts(rows_elem, sized):
+    """an empty chunk: tensors without elements have no address, buffers for the largest chunk have one"""
+    d, e, n = 64, 8, 4 if sized else 0
+    x = torch.empty((0, d), dtype=torch.float16, device="cuda")
+    idx, position = torch.empty((0, 2), dtype=torch.int32, device="cuda"), torch.empty((n, 2), dtype=torch.int32, device="cuda")
+    source, begin = torch.empty(2 * n, dtype=torch.int32, device="cuda"), torch.full((e + 1,), 5, dtype=torch.int32, device="cuda")
+    int8 = rows_elem == fmt.ELEM_I8
+    rows = torch.full((2 * n, d), 77, dtype=torch.int8 if int8 else torch.float16, device="cuda")
+    scales = torch.full((2 * n,), 77.0, device="cuda") if int8 else None
+    nv.sort_rows(idx, 0, 2, e, position, source, begin, x=x, d=d, rows=rows, rows_elem=rows_elem, row_scales=scales)
+    assert begin.tolist() == [0] * (e + 1) and (rows == 77).all()
+
+
 # ---- activations in their tails ----------------------------------------------------------------------------------
 
 def tails(rows, first, scale, up, activation, out):
