@@ -491,7 +491,8 @@ NVMAI_API int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_
 /* Gradients of merge_rows: drows[position[t][k]] = w[t][k] * dy[t] (rounded to `elem`; rows that no
  * position names are left as they were) and dw[t][k] = sum over i of dy[t][i] * rows[position[t][k]][i]
  * (fp32; 0 where the position is not held).  Positions are distinct, as sort_rows writes them (a row
- * that two pairs name gets the product of one of them).  w = NULL: weights of 1.  Either of drows and dw may be NULL;
+ * that two pairs name gets the product of one of them).  w = NULL: weights of 1.  Either of drows and dw may be NULL (both
+ * where there is nothing to write: no tokens, or no rows and no dw asked for);
  * rows may be NULL without dw; drows may be rows itself.  The gradient of base is dy. */
 NVMAI_API int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_stride, const void *rows,
                                              uint32_t rows_stride, uint32_t n_rows, const uint32_t *position,

@@ -669,7 +669,8 @@ int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_st
                                    uint32_t n_rows, const uint32_t *position, const void *w, uint32_t w_elem, uint32_t tokens,
                                    uint32_t top_k, uint32_t d, void *drows, uint32_t drows_stride, float *dw, void *stream) {
     return without_exceptions([&]() -> int {
-        if ((!drows && !dw) || (tokens != 0 && (!dy || !position))) return NVMAI_CUDA_EINVAL;
+        const bool nothing = tokens == 0 || (!dw && n_rows == 0);     // a buffer of no rows has no address
+        if ((!drows && !dw && !nothing) || (tokens != 0 && (!dy || !position))) return NVMAI_CUDA_EINVAL;
         if (dw && n_rows != 0 && !rows) return NVMAI_CUDA_EINVAL;
         if (elem > ELEM_BF16 || (w && w_elem > ELEM_BF16)) return NVMAI_CUDA_EINVAL;
         if (top_k == 0 || top_k > kRowMaxTopK || (uint64_t)tokens * top_k >= (1ull << 31) || d > kRowMaxLength) return NVMAI_CUDA_ERANGE;
@@ -678,7 +679,7 @@ int nvmai_cuda_moe_merge_rows_grad(const void *dy, uint32_t elem, uint32_t dy_st
         if (!aligned_to(dy, size) || !aligned_to(rows, size) || !aligned_to(drows, size) || (w && !aligned_to(w, elem_size(w_elem))) ||
             !aligned_to(dw, 4) || !aligned_to(position, 4))
             return NVMAI_CUDA_EINVAL;
-        if (tokens == 0) return NVMAI_CUDA_OK;
+        if (nothing) return NVMAI_CUDA_OK;
         const void *read = dw && n_rows != 0 ? rows : nullptr;       // the rows are read for dw alone
         if (!on_current_device({dy, read, position, w, n_rows != 0 ? drows : nullptr, dw})) return NVMAI_CUDA_EINVAL;
         const uint32_t pairs = tokens * top_k;
