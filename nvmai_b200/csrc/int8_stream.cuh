@@ -149,9 +149,12 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
             for (int x = 0; x < V; ++x) m = max(m, magnitude_bits(elem_to_float(v.v[x])));
             return m;
         };
-        // the first piece of up to four rows stays in registers; what else there is comes twice, the second time from the L1
+        // The first piece of up to three rows, or of one row of 16-byte pieces, is held between the two passes; what else there is comes
+        // twice, the second time from the L1.  As many as 64 registers leave room for beside the requested codes: with four rows held
+        // fp32 went through 64 bytes of local memory and bf16 through 14 (one row 2048 -> 2 x 512, four held / this: fp32 3.80 / 3.47 us,
+        // bf16 4.02 / 3.62, fp16 3.72 / 3.63; three rows of bf16 4.83 / 4.19; with two held one row 3.52, three rows of fp16 4.50 for 4.23).
         auto piece = [&](uint32_t r, uint32_t i) { return reinterpret_cast<const P *>(a + (size_t)r * p.a_stride)[i]; };
-        constexpr uint32_t kHeld = 4;
+        constexpr uint32_t kHeld = sizeof(P) > 8 ? 1 : 3;
         P held[kHeld];
         held[0] = early;
 #pragma unroll
