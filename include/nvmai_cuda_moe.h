@@ -482,7 +482,8 @@ NVMAI_API int nvmai_cuda_moe_sort_rows(const uint32_t *idx, uint32_t tokens, uin
 /* y[t] = base[t] + sum over k of w[t][k] * rows[position[t][k]]: expert rows back to their tokens,
  * in fp32 with k ascending, rounded once.  Positions >= n_rows add nothing, whatever their weight
  * is; w = NULL: weights of 1 (the gradient of sort_rows); base = NULL: 0.  rows, base and y have the type
- * `elem` (F16, F32, BF16), w has w_elem.  y may be base itself (the same rows in place). */
+ * `elem` (F16, F32, BF16), w has w_elem.  y may be base itself (the same rows in place).  top_k <= 64,
+ * tokens * top_k < 2^31 (the gradients' too); tokens = 0 and n_rows = 0 are valid. */
 NVMAI_API int nvmai_cuda_moe_merge_rows(const void *rows, uint32_t elem, uint32_t rows_stride, uint32_t n_rows,
                                         const uint32_t *position, const void *w, uint32_t w_elem, uint32_t tokens,
                                         uint32_t top_k, uint32_t d, const void *base, uint32_t base_stride, void *y,
@@ -534,8 +535,8 @@ NVMAI_API int nvmai_cuda_moe_int8_matmul(const void *a, uint32_t a_elem, uint32_
  * NVMAI_CUDA_EINVAL on a stream that is being captured. */
 NVMAI_API int nvmai_cuda_moe_int8_matmul_status(void *stream);
 
-/* Test hook for that failure path: the next int8_matmul call that runs on the tcgen05 kernel (more than 32 rows) with
- * k > 128 leaves out one copy, so its bounded waits run out.  Nothing faults or hangs. */
+/* Test hook for that failure path: the next int8_matmul call that runs on the tcgen05 kernel (every one of more than 64
+ * rows) with k > 128 leaves out one copy, so its bounded waits run out.  Nothing faults or hangs. */
 NVMAI_API int nvmai_cuda_moe_debug_drop_int8_copy(void);
 
 /* Optional per-kernel timeline of the single-token decode stages, the counterpart

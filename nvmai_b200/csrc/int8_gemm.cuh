@@ -5,9 +5,9 @@
 // of the same 128 features, so that one thread has both accumulators of an output).  Persistent: one block per SM, units in
 // the order (expert, channel tile, row tile), so that the row tiles that read the same codes run beside each other and the
 // codes cross HBM once.  Warps: 16 epilogue, 1 for the copies, 1 for the MMAs; the accumulators are double-buffered where two sets
-// fit.  By expert HBM bounds it: on a B200, 4096 tokens x 8 through 256 experts of 2048 -> 2 x 512 take 110 us (5.8 TB/s; 126 in a loop
-// of seconds under the power cap, where leaving out three MMAs of four gave 109), 201 tokens of 512 -> 2048 45 us (6.2 TB/s).  One matrix of
-// 2048 -> 2 x 1024 and 16384 rows: 54 us, 2.5 x 10^15 operations a second.
+// fit.  By expert HBM bounds it: on a B200, 4096 tokens x 8 through 256 experts of 2048 -> 2 x 512 take 110 us (5.8 TB/s; 116 to 126
+// in loops of seconds under the power cap, where leaving out three MMAs of four gave 109), 201 tokens of 512 -> 2048 45 us (6.2 TB/s).
+// One matrix of 2048 -> 2 x 1024 and 16384 rows: 55 us, 2.5 x 10^15 operations a second (59 with three sets of rows in turn).
 #pragma once
 #include <type_traits>
 

@@ -86,13 +86,15 @@ IgTile cheapest_tile(const Matmul &m, uint32_t experts, float rows) {
     return best;
 }
 
-// One matrix, or one for each expert.  Where every SM has several units HBM is the limit: the codes come once for each unit of an
-// expert (past the first from the L2), so a unit holds the average expert and 2.5 times the spread of an even routing around
-// it.  Past 128 rows that leaves one set of accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 118.0 us, 160
-// 110.5, 192 113.7 (three ring slots instead of four); 512 -> 2048: 72.6, 69.7, 67.7.  Two channel tiles a unit read the rows half
-// as often: 201 tokens, 512 -> 2048, 54.1 us with one, 46.7 with two.  Below three units an SM the model picks, for the average
-// and twice the spread: 41 tokens x 8 through 8 experts of 1711 -> 596 12.3 us with the rule above, 9.0 with the model; 201 x 8
-// through 16 of 2048 -> 2 x 512 14.1 / 12.2; 1000 x 8 through 64 of those 31.9 / 32.1.
+// One matrix, or one for each expert.  With three units an SM or more (counted for all experts, those without rows too), the rule is
+// made for many experts, where HBM is the limit: the codes come once for each unit of an expert (past the first from the L2), so a
+// unit holds the average expert and 2.5 times the spread of an even routing around it.  Past 128 rows that leaves one set of
+// accumulators; 256 experts of 128 rows on average, 2048 -> 2 x 512: 128 rows a unit 114.1 us, 160 106.0, 192 106.6 (three ring slots
+// instead of four); 512 -> 2048: 76.2, 70.0, 69.6.  Two channel tiles a unit read the rows half as often: 201 tokens, 512 -> 2048,
+// 52.6 us with one, 45.4 with two.  Below three units an SM the model picks, for the average and twice the spread: 41 tokens x 8
+// through 8 experts of 1711 -> 596 10.9 us with the rule above, 7.4 to 8.1 with the model; 201 x 8 through 16 of 2048 -> 2 x 512
+// 13.4 / 12.0; 1000 x 8 through 64 of those 34.8 / 35.4.  Few large experts are bound by the operations, which the rule does not
+// know: 4096 x 8 through 8 of those 66.2 us with it, 61.4 with the model, 512 -> 2048 51 / 48; through 64 75.9 / 74.1 and 53.8 / 55.5.
 IgTile row_tile(const Matmul &m) {
     if (m.begin == nullptr) return cheapest_tile(m, 1, (float)m.rows);
     const float average = (float)m.rows / (float)m.E;
@@ -140,18 +142,18 @@ cudaError_t launch_gemm(const Matmul &m, cudaStream_t st) {
 }
 
 // The streaming kernel's tiles of 8 rows, 0: the tcgen05 kernel's.  One matrix: up to 16 rows, up to 32 where the tcgen05 kernel would
-// go through eight K blocks or more one after the other (codes on a B200, streaming / tcgen05: 2048 -> 2 x 512, 1 row 3.1 / 7.6 us,
-// 16 rows 4.1 / 7.6, 32 rows 5.9 / 7.7; 512 -> 2048, 16 rows 3.1 / 3.9, 32 rows 4.3 / 4.0; 1024 -> 1024, 32 rows 4.2 / 4.7).  By
-// expert a block has the rows of one, and every one fetches its codes anew: while rows x k is below 2^15 (8 rows of 2048: 6.7 /
-// 10.7 us, 16 rows 11.7 / 12.1, 24 rows 16.2 / 14.4; 32 rows of 512 10.5 / 10.5, 64 rows 17.3 / 15.0).
+// go through eight K blocks or more one after the other (codes on a B200, streaming / tcgen05: 2048 -> 2 x 512, 1 row 2.9 / 8.1 us,
+// 16 rows 4.2 / 8.1, 32 rows 5.9 / 8.3; 512 -> 2048, 16 rows 3.2 / 4.1, 32 rows 4.2 / 4.2; 1024 -> 1024, 32 rows 4.3 / 4.9).  By
+// expert a block has the rows of one, and every one fetches its codes anew: while rows x k is below 2^15 (8 rows of 2048: 5.4 /
+// 9.8 us, 16 rows 10.9 / 10.4, 24 rows 15.4 / 12.4; 16 rows of 512 4.9 / 6.1, 32 rows 9.9 / 9.7, 64 rows 16.3 / 14.0).
 uint32_t stream_tiles(const Matmul &m) {
     if (m.begin != nullptr ? (uint64_t)m.rows * m.k >= 32768 || m.rows > 64 : m.rows > (m.k >= 1024 ? 32u : 16u)) return 0;
     const uint32_t nt = m.begin != nullptr || m.rows <= 8 ? 1 : m.rows <= 16 ? 2 : 4;
     return is_smem(m.k, nt) <= 200 * 1024 ? nt : 0;
 }
 // Does it quantise the rows itself?  Each of its blocks then does, 0.3 us a row of 2048 in front of the product; a launch for all of
-// them runs beside the fetching of the codes, and costs the host 2.4 us (2048 -> 2 x 512, one launch / two: 1 row 3.7 / 4.3 us, 3
-// rows 4.3 / 4.3, 4 rows 4.8 / 4.3; 3 rows of 4096 6.5 / 5.0; one token through eight experts 7.3 / 7.4).
+// them runs beside the fetching of the codes, and costs the host 2.4 us (2048 -> 2 x 512, one launch / two: 1 row 3.6 / 4.4 us, 3
+// rows 4.2 / 4.2, 4 rows 4.9 / 4.2; 3 rows of 4096 6.2 / 4.9; one token through eight experts 6.2 / 6.3).
 bool stream_quantizes(const Matmul &m) { return m.begin != nullptr || (m.rows <= 4 && m.rows * m.k <= 6144); }
 
 cudaError_t launch_stream(const Matmul &m, uint32_t nt, cudaStream_t st) {

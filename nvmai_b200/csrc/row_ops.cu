@@ -20,13 +20,13 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // A stable counting sort: the row of a pair is (kept pairs of smaller experts) + (pairs of its expert in front of it).  Each
 // block has a run of tokens; it counts the experts of all pairs, those in front of its run apart, and ranks its own pairs
 // with one warp, 32 at a time (__match_any_sync gives the pairs of the same expert).  Then its warps move the tokens' rows.  Writing
-// bounds it: 4096 tokens of 4 KB to eight experts each take 32.3 us on a B200, 5.9 of them for the order (the same 134 MB written in order
-// take 24.6); one token 3.0.
+// bounds it: 4096 tokens of 4 KB to eight experts each take 33.2 us on a B200, 5.9 of them for the order (the same 134 MB written in order
+// take 24.6); one token 3.1.
 constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kSms = 148, kSortBlocks = kSms;
 constexpr uint32_t kSortOwn = 4096;          // most pairs of a block: their experts and rows are in shared memory
-// From this many pairs on the blocks' counts come from a kernel in front (the order alone on a B200, top-8 of 256: 8192 tokens 10.3
-// us with all pairs counted by every block, 9.4 with that kernel; 16384 tokens 18.0 / 13.3; 65536 tokens 57 / 28).
+// From this many pairs on the blocks' counts come from a kernel in front (the order alone on a B200, top-8 of 256: 8192 tokens 10.0
+// us with all pairs counted by every block, 9.5 with that kernel; 16384 tokens 18.2 / 13.9; 65536 tokens 66.6 / 34.0).
 constexpr uint32_t kSortCounted = 65536;
 
 struct SortParams {
@@ -245,7 +245,7 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int byte
 // A warp sums a run of 32 R pieces of V neighbouring elements of a token and goes on to the next run, as many warps further as
 // there are.  A step is a run's pieces of up to eight slots; a step is copied into shared memory while the one before is
 // added, each lane its own pieces, so that a lane waits for its own copies alone (cp.async groups) and no registers hold what is
-// in flight: 24 warps an SM with a step of 4 KB each.  4096 tokens of eight 4 KB rows on a B200: 25.4 us, 5.9 TB/s; a thread per piece
+// in flight: 24 warps an SM with a step of 4 KB each.  4096 tokens of eight 4 KB rows on a B200: 25.1 us, 6.0 TB/s; a thread per piece
 // without the ring 35.2 (the rows' latency is exposed), a ring of four steps 56 (8 warps an SM, too few for the instructions).
 constexpr uint32_t kMergeSlots = 8, kMergeAhead = 2;
 __host__ __device__ constexpr uint32_t merge_stage_bytes(uint32_t top_k, uint32_t run_bytes) {
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(MergeParams p) {
 }
 
 // Rows of 16-bit elements that share no 4-byte boundary: a thread sums every 32nd element, four of them and four slots at a time
-// (two-byte accesses bound it: 1531 tokens of eight rows of 999 elements 14.4 us on a B200, 1.9 TB/s).
+// (two-byte accesses bound it: 1531 tokens of eight rows of 999 elements 11.3 us on a B200, 2.4 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) merge_narrow_kernel(MergeParams p) {
     constexpr int U = 4, kAhead = 4;
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(256, 4) merge_rows_grad_kernel(MergeGradParams
     const P *v = reinterpret_cast<const P *>(static_cast<const T *>(p.rows) + (size_t)row * p.rows_stride);
     P *o = reinterpret_cast<P *>(static_cast<T *>(p.drows) + (size_t)row * p.drows_stride);
     // kAhead pieces of both rows are requested before any is stored: drows may be rows, so the compiler keeps loads behind stores.
-    // 1531 tokens of 2048 bf16 elements on a B200: two pieces and 32 warps an SM 21.4 us, three and 24 warps 23.1, two and 40 24.7.
+    // 1531 tokens of 2048 bf16 elements on a B200: two pieces and 32 warps an SM 21.6 us, three and 24 warps 23.1, two and 40 24.7.
     constexpr int kAhead = V == 8 ? 2 : V == 4 ? 4 : 8;
     const uint32_t pieces = p.d / V;
     float dot = 0.0f;
