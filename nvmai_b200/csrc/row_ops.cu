@@ -570,7 +570,7 @@ cudaError_t nvmai::launch_quantize(const void *x, uint32_t elem, uint32_t x_stri
         // 201 x 2048 2.5 / 2.0, 1000 x 2048 2.6 / 3.6, 32768 x 512 12.8 / 67.7, 300 x 8000 13.1 / 3.4)
         if (rows < 3 * kSms || n > 32u * kQuantizeHeld * v)
             return launch_pdl(quantize_rows_kernel<decltype(T), v, 8>, dim3(rows), dim3(256), 0, st, true, p);
-        return launch_pdl(quantize_rows_kernel<decltype(T), v, 1>, dim3((rows + 7) / 8), dim3(256), 0, st, true, p);
+        return launch_pdl(quantize_rows_kernel<decltype(T), v, 1>, dim3(rows / 8 + (rows % 8 != 0)), dim3(256), 0, st, true, p);
     });
 }
 

@@ -265,3 +265,18 @@ def test_products_of_matrices_and_outputs_past_32_bits(rows):
         assert torch.equal(out[r * far_out:r * far_out + n], near[r])
     del wide, out
     torch.cuda.empty_cache()
+
+
+def test_codes_of_four_billion_rows():
+    """as many rows as the count's 32 bits hold: the last block's are not lost in a sum past them"""
+    rows = 0xFFFFFFFF
+    x = torch.zeros(rows, dtype=torch.float16, device="cuda")
+    x[-3:], x[0] = torch.tensor([2.0, -127.0, 0.5]), 1.0
+    q, s = torch.full((rows,), 77, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    nv.quantize_rows(x, rows, 1, q, s)
+    want, scale = codes64(torch.stack([x[0], *x[-4:]])[:, None])
+    at = torch.tensor([0, rows - 4, rows - 3, rows - 2, rows - 1], device="cuda")
+    assert torch.equal(q[at].double(), want[:, 0]) and torch.equal(s[at].double(), scale)
+    assert int(q.count_nonzero()) == 4
+    del x, q, s
+    torch.cuda.empty_cache()
