@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kIsThreads, NT == 1 ? 2 : 1) int8_stream_kerne
         // twice, the second time from the L1.  As many as 64 registers leave room for beside the requested codes: with four rows held
         // fp32 went through 64 bytes of local memory and bf16 through 14 (one row 2048 -> 2 x 512, four held / this: fp32 3.80 / 3.47 us,
         // bf16 4.02 / 3.62, fp16 3.72 / 3.63; three rows of bf16 4.83 / 4.19; with two held one row 3.52, three rows of fp16 4.50 for 4.23).
+        // What is left of it: 16 to 32 bytes with fp32, 2 with bf16.
         auto piece = [&](uint32_t r, uint32_t i) { return reinterpret_cast<const P *>(a + (size_t)r * p.a_stride)[i]; };
         constexpr uint32_t kHeld = sizeof(P) > 8 ? 1 : 3;
         P held[kHeld];
